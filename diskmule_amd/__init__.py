@@ -16,6 +16,8 @@ from .hip import (  # noqa: F401
     ExpertCache,
     ExpertLayerLayout,
     KvLayer,
+    KvPages,
+    KvPlan,
     BackendSelection,
     library_path,
     load_library,

@@ -22,7 +22,7 @@ LIB = os.path.join(HERE, "libdmhip.so")
 DIAG_LIB = os.path.join(HERE, "libdmhip_diag.so")
 SOURCES = ["runtime.hip", "dispatch.hip", "kernels_simple.hip", "kernels_qmv.hip", "kernels_qmv8.hip",
            "kernels_gemm.hip", "expert_cache.hip", "kernels_dense.hip", "attention.hip",
-           "kernels_safetensor.hip"]
+           "kernels_safetensor.hip", "kv_pages.hip", "attn_pages.hip"]
 DIAG_SOURCES = ["diag/probes.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",

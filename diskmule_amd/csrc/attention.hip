@@ -966,7 +966,7 @@ const void *module_anchor_attention() { return (const void *)attn_combine_kernel
 
 // ---- validation, same checks in the same order as src/metal.rs ----
 
-static int fail_shape(const char *reason) {
+int fail_shape(const char *reason) {
     fail(DMHIP_ERR_INVALID_ATTENTION_SHAPE, "invalid attention shape: %s", reason);
     last_detail().reason = reason;
     return DMHIP_ERR_INVALID_ATTENTION_SHAPE;
@@ -986,7 +986,7 @@ static int fail_kv_width(size_t expected, size_t actual) {
     return DMHIP_ERR_KV_WIDTH;
 }
 
-static int fail_kv_context(size_t position, size_t limit) {
+int fail_kv_context(size_t position, size_t limit) {
     fail(DMHIP_ERR_KV_CONTEXT, "HIP KV cache position %zu exceeds its context limit %zu", position, limit);
     last_detail().position = position;
     last_detail().limit = limit;
@@ -1030,6 +1030,12 @@ static int check_kernel_limits(size_t query_heads, size_t kv_heads, size_t hd, s
 static uint32_t next_mark(dmhip_ctx *ctx) {
     ctx->attn_mark = ctx->attn_mark + 1 ? ctx->attn_mark + 1 : 1;
     return ctx->attn_mark;
+}
+
+BadFlag attention_device_flag(dmhip_ctx *ctx) {
+    // the device calls between two results share one mark, so the result
+    // reports a non-finite score in any of them
+    return BadFlag{ctx->flags + kAttnFlagWord, ctx->attn_pending ? ctx->attn_mark : next_mark(ctx)};
 }
 
 // The mark of a host-slice call: it ends the period of device calls awaiting
@@ -1222,12 +1228,9 @@ int dmhip_attention_cached_device(dmhip_ctx *ctx, const float *query_device, siz
     const size_t start = layer->position - visible;
     DM_CHECK_STATUS(check_kernel_limits(query_heads, kv_heads, head_dimension, visible));
     DM_CHECK_STATUS(set_device(ctx));
-    // the device calls between two results share one mark, so the result
-    // reports a non-finite score in any of them
-    const uint32_t mark = ctx->attn_pending ? ctx->attn_mark : next_mark(ctx);
     DM_CHECK_STATUS(enqueue_attention(ctx, query_device, layer->keys, layer->values, layer->capacity,
                                       layer->width, query_heads, kv_heads, head_dimension, start, visible,
-                                      output_device, BadFlag{ctx->flags + kAttnFlagWord, mark}));
+                                      output_device, attention_device_flag(ctx)));
     ctx->attn_pending = true;
     return DMHIP_OK;
 }
@@ -1235,7 +1238,7 @@ int dmhip_attention_cached_device(dmhip_ctx *ctx, const float *query_device, siz
 int dmhip_attention_result(dmhip_ctx *ctx) {
     DM_REQUIRE_PTR(ctx);
     if (!ctx->attn_pending)
-        return fail(DMHIP_ERR_INVALID_ARGUMENT, "no dmhip_attention_cached_device call awaits its result");
+        return fail(DMHIP_ERR_INVALID_ARGUMENT, "no device attention call awaits its result");
     DM_CHECK_STATUS(set_device(ctx));
     uint32_t flag = 0;
     DM_HIP(hipMemcpyAsync(&flag, ctx->flags + kAttnFlagWord, 4, hipMemcpyDeviceToHost, ctx->stream));

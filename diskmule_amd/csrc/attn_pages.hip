@@ -1,0 +1,539 @@
+// attn_pages.hip -- attention over a paged KV cache: whole prompts, decode
+// steps of a batch and sequences that share a prefix are all lists of units
+// (dm_pages.h), each some query rows of one KV head against a range of one
+// sequence's positions.
+//
+// For query row r at position p and the positions j it sees (j <= p, and
+// j > p - window where there is one): x_j = scale * q_r . k_j and
+// o_r = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m), x in units of log2 and m any
+// number near the largest x: one pass over the keys and values with a running
+// m, sum and o.  Units over parts of a row's positions leave (m, sum, o), which
+// join_kernel brings to one m and adds.
+#include <math.h>
+
+#include "dm_device.h"
+#include "kv_pages.h"
+
+namespace dm {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr uint32_t kSplitWaves = 4;
+
+// A page type's products: A is 16 keys (or 16 dims of values) by 32, B is 32
+// by 16 rows; lane l holds A's row and B's column l % 16, elements 8 (l / 16)
+// .. + 7, and of the result column l % 16, rows 4 (l / 16) .. + 3.
+template <bool BF>
+struct Page;
+template <>
+struct Page<true> {
+    typedef __bf16 T;
+    static __device__ __forceinline__ floatx4 mfma(u32x4 a, u32x4 b, floatx4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    }
+};
+template <>
+struct Page<false> {
+    typedef _Float16 T;
+    static __device__ __forceinline__ floatx4 mfma(u32x4 a, u32x4 b, floatx4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0,
+                                                      0, 0);
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(T lo, T hi) {
+    return (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
+}
+
+__device__ __forceinline__ float load_one(const void *p, uint32_t type, uint64_t i) {
+    if (type == kF32) return ((const float *)p)[i];
+    const uint16_t b = ((const uint16_t *)p)[i];
+    return type == kBF16 ? __uint_as_float((uint32_t)b << 16) : (float)__builtin_bit_cast(_Float16, b);
+}
+
+// Eight consecutive values, of any alignment their type allows.
+__device__ __forceinline__ void load_eight(const void *p, uint32_t type, uint64_t i, float *v) {
+    if (type == kF32) {
+        const f32x4a4 a = *(const f32x4a4 *)((const float *)p + i), b = *(const f32x4a4 *)((const float *)p + i + 4);
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = a[k], v[k + 4] = b[k];
+        return;
+    }
+    const u32x4a2 w = *(const u32x4a2 *)((const uint16_t *)p + i);
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if (type == kBF16) {
+            v[2 * k] = __uint_as_float(w[k] << 16);
+            v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+        } else {
+            v[2 * k] = (float)__builtin_bit_cast(_Float16, (uint16_t)w[k]);
+            v[2 * k + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[k] >> 16));
+        }
+    }
+}
+
+__device__ __forceinline__ void store_one(void *p, uint32_t type, uint64_t i, float v) {
+    if (type == kF32)
+        ((float *)p)[i] = v;
+    else if (type == kBF16)
+        ((__bf16 *)p)[i] = (__bf16)v;
+    else
+        ((_Float16 *)p)[i] = (_Float16)v;
+}
+
+__device__ __forceinline__ void store_four(void *p, uint32_t type, uint64_t i, floatx4 v) {
+    typedef uint32_t u32x2a2 __attribute__((ext_vector_type(2), aligned(2)));
+    if (type == kF32) {
+        *(f32x4a4 *)((float *)p + i) = v;
+        return;
+    }
+    u32x2a2 w;
+    if (type == kBF16)
+        w = u32x2a2{pack2((__bf16)v[0], (__bf16)v[1]), pack2((__bf16)v[2], (__bf16)v[3])};
+    else
+        w = u32x2a2{pack2((_Float16)v[0], (_Float16)v[1]), pack2((_Float16)v[2], (_Float16)v[3])};
+    *(u32x2a2 *)((uint16_t *)p + i) = w;
+}
+
+__device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
+
+// 2^x as the hardware has it: within 1 ulp, results below 2^-126 are zero.
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Loads stay on their side of this: the registers of a wide head hold a group
+// of operands at a time, not all that could be asked for at once.
+__device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
+
+// The positions a query at `position` sees: [lo, hi).
+__device__ __forceinline__ void seen(const AttnCall &c, uint32_t position, uint32_t &lo, uint32_t &hi) {
+    hi = position + 1;
+    lo = c.window && hi > c.window ? hi - c.window : 0;
+}
+
+struct RowAt {
+    uint32_t token, head;  // query head
+};
+__device__ __forceinline__ RowAt row_at(const AttnCall &c, uint32_t row, uint32_t h) {
+    const uint32_t t = row / c.group;
+    return {t, h * c.group + (row - t * c.group)};
+}
+
+__device__ __forceinline__ const PlanHeader &head_of(const AttnCall &c) { return *(const PlanHeader *)c.plan; }
+
+// Rows of a unit again, with every masked product left out instead of multiplied by
+// zero, and queries and probabilities in 32 bits: for rows that met a value that
+// is not finite (marked in `again`).  Such a value in a place that a row does not see must
+// not reach its result (0 * inf), and where queries or probabilities are split
+// into terms, one that it does see gives inf - inf.  One wave a row: a lane a
+// key, then a lane a dim.
+template <bool BF>
+__device__ void careful_rows(const AttnCall &c, const AttnUnit &u, uint32_t h, uint32_t waves, const uint32_t *again) {
+    typedef typename Page<BF>::T T;
+    const uint32_t lane = threadIdx.x & 63u, hd = c.kv.head_dim;
+    const uint32_t *positions = (const uint32_t *)(c.plan + head_of(c).position_at);
+    for (uint32_t r = threadIdx.x >> 6; r < u.rows; r += waves) {
+        if (!again[r]) continue;
+        const RowAt at = row_at(c, u.row0 + r, h);
+        uint32_t lo, hi;
+        seen(c, positions[at.token], lo, hi);
+        const uint64_t q0 = at.token * c.q_stride + (uint64_t)at.head * hd;
+        float m = -INFINITY, l = 0.0f, o[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) o[k] = 0.0f;
+        for (uint32_t t0 = u.kv0; t0 < u.kv1; t0 += 64) {
+            const uint32_t page = c.kv.table[(uint64_t)u.seq * c.kv.row + t0 / kPageTokens];
+            const T *kp = (const T *)c.kv.base + ((uint64_t)page * c.kv.kv_heads + h) * 2 * hd * kPageTokens;
+            const T *vp = kp + hd * kPageTokens;
+            const uint32_t t = t0 + lane;
+            const bool in = t >= lo && t < hi && t < u.kv1;
+            if (!__any(in)) continue;
+            float x = -INFINITY;
+            if (in) {
+                float s = 0.0f;
+                for (uint32_t d = 0; d < hd; d++)
+                    s = __builtin_fmaf(load_one(c.q, c.q_type, q0 + d), (float)kp[((d >> 3) * 64 + lane) * 8 + (d & 7)], s);
+                x = s * c.scale;
+            }
+            float top = x;
+#pragma unroll
+            for (int k = 32; k >= 1; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
+            const float next = fmaxf(m, top), from = next == -INFINITY ? 0.0f : next;
+            const float keep = exp2_hw(m - from), p = in ? exp2_hw(x - from) : 0.0f;
+            l = l * keep + wave_sum(p);
+#pragma unroll
+            for (int k = 0; k < 8; k++) o[k] = keep == 1.0f ? o[k] : o[k] * keep;
+            m = next;
+            for (uint32_t k = 0; k < 64; k++) {
+                const float w = __shfl(p, (int)k, 64);
+                if (!__shfl((int)in, (int)k, 64) || w == 0.0f) continue;
+                const uint32_t chunk = 2 * (k >> 4) + ((k >> 2) & 1), j = ((k >> 3) & 1) * 4 + (k & 3);
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e++) {
+                    const uint32_t d = e * 64 + lane;
+                    if (d < hd) o[e] = __builtin_fmaf(w, (float)vp[(chunk * hd + d) * 8 + j], o[e]);
+                }
+            }
+        }
+        if (u.part == kNoPart) {
+            if (lane == 0 && !(l > 0.0f)) *c.bad.word = c.bad.mark;
+        } else if (lane == 0) {
+            c.part_ml[(uint64_t)(u.part + r) * c.kv.kv_heads + h] = float2{m, l};
+        }
+#pragma unroll
+        for (uint32_t e = 0; e < 8; e++) {
+            const uint32_t d = e * 64 + lane;
+            if (d >= hd) continue;
+            if (u.part == kNoPart)
+                store_one(c.out, c.out_type, at.token * c.out_stride + (uint64_t)at.head * hd + d, o[e] / l);
+            else
+                c.part_o[((uint64_t)(u.part + r) * c.kv.kv_heads + h) * hd + d] = o[e];
+        }
+    }
+}
+
+// Units of up to 16 NB rows.  The waves share the positions: each takes every
+// fourth block of 32, reads its keys and values once from memory straight into
+// the matrix operands, and uses them for all rows, so that a unit reads what
+// its rows see once; the waves' results meet in LDS at the end.
+//
+// EXACT (32-bit results): queries and probabilities in two halves (F16) or
+// three and two (BF16), which leaves 2^-17 of a probability; otherwise each is
+// rounded to the page type once, half a step of it, as the result is.
+template <bool BF, int D, int NB, bool EXACT>
+__global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c, uint32_t cls) {
+    typedef typename Page<BF>::T T;
+    constexpr int kRows = 16 * NB, KS = D / 32, DB = D / 16;
+    constexpr int QT = EXACT ? (BF ? 3 : 2) : 1, PT = EXACT ? 2 : 1;
+    // Probabilities of F16 pages are 2^10 times larger: its smallest value 2^-24
+    // would lose the many small ones of a long row.
+    constexpr float kLift = BF ? 0.0f : 10.0f;
+    constexpr int kReducePitch = 36;  // floats of a row of 32 dims: rows start 4 banks apart
+    constexpr int kQueryBytes = QT * NB * KS * 64 * 16;
+    constexpr int kReduceBytes = kSplitWaves * kRows * kReducePitch * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t shared[kQueryBytes > kReduceBytes ? kQueryBytes : kReduceBytes];
+    __shared__ float row_scale[kRows];
+    __shared__ float2 wave_ml[kSplitWaves][kRows];
+    __shared__ uint32_t again[kRows], any_again;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, n16 = lane & 15u, g = lane >> 4;
+    const uint32_t hd = c.kv.head_dim, kvh = c.kv.kv_heads;
+    const PlanHeader &head = head_of(c);
+    const AttnUnit *units = (const AttnUnit *)(c.plan + head.unit_at[cls]);
+    const uint32_t *positions = (const uint32_t *)(c.plan + head.position_at);
+    const uint32_t total = head.unit_count[cls] * kvh;
+
+    for (uint32_t job = blockIdx.x; job < total; job += gridDim.x) {
+        const uint32_t h = job % kvh;
+        const AttnUnit u = units[job / kvh];
+        if (tid < kRows) again[tid] = 0;
+        if (tid == 0) any_again = 0;
+        // ---- queries into LDS, as the B operands of the products ----
+        {
+            constexpr int kPer = 64 * kSplitWaves / kRows;  // threads of a row, in one wave
+            const uint32_t r = tid / kPer, sub = tid % kPer;
+            const bool there = r < u.rows;
+            const RowAt at = row_at(c, u.row0 + (there ? r : 0), h);
+            const uint64_t q0 = at.token * c.q_stride + (uint64_t)at.head * hd;
+            int e = 0;
+            if (!BF && c.q_type == kF32) {
+                // F16 terms of a 32-bit query: its row by a power of two that
+                // brings the largest to 2^14, so that none overflows and the
+                // second half of a small one is still there
+                float top = 0.0f;
+                if (there)
+                    for (uint32_t ch = sub; ch < hd / 8; ch += kPer) {
+                        float v[8];
+                        load_eight(c.q, c.q_type, q0 + ch * 8, v);
+#pragma unroll
+                        for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(v[k]));
+                    }
+#pragma unroll
+                for (int k = kPer / 2; k >= 1; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
+                if (top > 0.0f && finite(top)) e = (int)(__float_as_uint(top) >> 23) - 127 - 14;
+            }
+            if (sub == 0) row_scale[r] = ldexpf(c.scale, e);
+#pragma unroll 1
+            for (uint32_t ch = sub; ch < D / 8; ch += kPer) {
+                float v[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] = 0.0f;
+                if (there && ch < hd / 8) load_eight(c.q, c.q_type, q0 + ch * 8, v);
+                if (!BF && e != 0) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) v[k] = ldexpf(v[k], -e);
+                }
+                const uint32_t slot = (((r >> 4) * KS + (ch >> 2)) * 64 + (ch & 3) * 16 + (r & 15)) * 16;
+#pragma unroll
+                for (int term = 0; term < QT; term++) {
+                    T t[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        t[k] = (T)v[k];
+                        v[k] = v[k] - (float)t[k];
+                    }
+                    *(u32x4 *)(shared + term * (NB * KS * 1024) + slot) =
+                        u32x4{pack2(t[0], t[1]), pack2(t[2], t[3]), pack2(t[4], t[5]), pack2(t[6], t[7])};
+                }
+            }
+        }
+        __syncthreads();
+
+        float scale[NB];
+        uint32_t lo[NB], hi[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+            const uint32_t r = nb * 16 + n16;
+            scale[nb] = row_scale[r];
+            lo[nb] = 0;
+            hi[nb] = 0xffffffffu;
+            if (r < u.rows) seen(c, positions[(u.row0 + r) / c.group], lo[nb], hi[nb]);
+        }
+        floatx4 acc[DB][NB];
+#pragma unroll
+        for (int db = 0; db < DB; db++)
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) acc[db][nb] = floatx4{0, 0, 0, 0};
+        // m: what the running sum and o are relative to; l: this lane's share
+        float m[NB], l[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) m[nb] = -INFINITY, l[nb] = 0.0f;
+
+        const uint32_t *table = c.kv.table + (uint64_t)u.seq * c.kv.row;
+        const uint32_t blocks = (u.kv1 + 31) / 32;
+#pragma unroll 1
+        for (uint32_t b = u.kv0 / 32 + wave; b < blocks; b += kSplitWaves) {
+            const uint32_t page = (uint32_t)__builtin_amdgcn_readfirstlane((int)table[b >> 1]);
+            const T *kp = (const T *)c.kv.base + ((uint64_t)page * kvh + h) * 2 * hd * kPageTokens;
+            const T *vp = kp + hd * kPageTokens + ((b & 1) * 4 + g) * hd * 8;
+            // Scores of 32 keys: row 4 g + i of half a is key
+            // 16 (g / 2) + 4 (g % 2) + i + 8 a, so that a lane's eight are the
+            // tokens of one value chunk, in its order.
+            const T *kl = kp + ((b & 1) * 32 + 16 * (n16 >> 3) + 4 * ((n16 >> 2) & 1) + (n16 & 3)) * 8;
+            floatx4 s[2][NB];
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) s[0][nb] = s[1][nb] = floatx4{0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                if (ks % 4 == 0) in_order();
+                const uint32_t ch = ks * 4 + g;
+                u32x4 k0 = {0, 0, 0, 0}, k1 = {0, 0, 0, 0};
+                if (ch * 8 < hd) {
+                    k0 = *(const u32x4 *)(kl + ch * 512);
+                    k1 = *(const u32x4 *)(kl + ch * 512 + 64);
+                }
+#pragma unroll
+                for (int term = 0; term < QT; term++)
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++) {
+                        const u32x4 q = *(const u32x4 *)(shared + (((term * NB + nb) * KS + ks) * 64 + lane) * 16);
+                        s[0][nb] = Page<BF>::mfma(k0, q, s[0][nb]);
+                        s[1][nb] = Page<BF>::mfma(k1, q, s[1][nb]);
+                    }
+            }
+            const uint32_t t0 = b * 32;
+            u32x4 p[PT][NB];
+            const bool whole = t0 >= u.full0 && t0 + 32 <= u.full1;
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) {
+                float x[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] = s[k >> 2][nb][k & 3] * scale[nb];
+                if (!whole) {
+                    const uint32_t first = t0 + 16 * (g >> 1) + 4 * (g & 1);
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const uint32_t t = first + (k & 3) + 8 * (k >> 2);
+                        x[k] = t >= lo[nb] && t < hi[nb] ? x[k] : -INFINITY;
+                    }
+                }
+                float top = x[0];
+#pragma unroll
+                for (int k = 1; k < 8; k++) top = fmaxf(top, x[k]);
+                // m follows the largest score only when that is 5 above it:
+                // until then the sum and o stay as they are
+                constexpr float kSlack = 5.0f;
+                if (__any(top > m[nb] + kSlack)) {
+                    top = fmaxf(top, __shfl_xor(top, 16, 64));
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    const float next = fmaxf(m[nb], top);
+                    const float keep = m[nb] == next ? 1.0f : exp2_hw(m[nb] - next);
+                    m[nb] = next;
+                    l[nb] *= keep;
+#pragma unroll
+                    for (int db = 0; db < DB; db++) acc[db][nb] = acc[db][nb] * keep;
+                }
+                const float from = (m[nb] == -INFINITY ? 0.0f : m[nb]) - kLift;
+                T t[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    x[k] = exp2_hw(x[k] - from);
+                    l[nb] += x[k];
+                }
+#pragma unroll
+                for (int term = 0; term < PT; term++) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        t[k] = (T)x[k];
+                        x[k] = x[k] - (float)t[k];
+                    }
+                    p[term][nb] = u32x4{pack2(t[0], t[1]), pack2(t[2], t[3]), pack2(t[4], t[5]), pack2(t[6], t[7])};
+                }
+            }
+#pragma unroll
+            for (int db = 0; db < DB; db++) {
+                if (db % 8 == 0) in_order();
+                const uint32_t d = db * 16 + n16;
+                const u32x4 v = *(const u32x4 *)(vp + (d < hd ? d : hd - 1) * 8);
+#pragma unroll
+                for (int term = 0; term < PT; term++)
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++) acc[db][nb] = Page<BF>::mfma(v, p[term][nb], acc[db][nb]);
+            }
+        }
+
+        // ---- the waves' results to one m, added ----
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+            l[nb] += __shfl_xor(l[nb], 16, 64);
+            l[nb] += __shfl_xor(l[nb], 32, 64);
+            if (g == 0) wave_ml[wave][nb * 16 + n16] = float2{m[nb], l[nb]};
+        }
+        __syncthreads();  // and all queries read: their place is used again
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+            float top = -INFINITY;
+#pragma unroll
+            for (uint32_t w = 0; w < kSplitWaves; w++) top = fmaxf(top, wave_ml[w][nb * 16 + n16].x);
+            const float f = m[nb] == top ? 1.0f : exp2_hw(m[nb] - top);
+#pragma unroll
+            for (int db = 0; db < DB; db++) acc[db][nb] = acc[db][nb] * f;
+        }
+        float *reduce = (float *)shared;
+#pragma unroll
+        for (int dc = 0; dc < D / 32; dc++) {
+            if (dc) __syncthreads();
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+                    *(floatx4 *)(reduce + (wave * kRows + nb * 16 + n16) * kReducePitch + k * 16 + g * 4) =
+                        acc[dc * 2 + k][nb];
+            __syncthreads();
+            for (uint32_t i = tid; i < kRows * 8; i += 64 * kSplitWaves) {
+                const uint32_t r = i >> 3, d = dc * 32 + (i & 7) * 4;
+                if (r >= u.rows || d >= hd) continue;
+                float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+                for (uint32_t w = 0; w < kSplitWaves; w++) top = fmaxf(top, wave_ml[w][r].x);
+#pragma unroll
+                for (uint32_t w = 0; w < kSplitWaves; w++) {
+                    const float2 ml = wave_ml[w][r];
+                    sum += ml.x == top ? ml.y : ml.y * exp2_hw(ml.x - top);
+                }
+                floatx4 o = {0, 0, 0, 0};
+#pragma unroll
+                for (uint32_t w = 0; w < kSplitWaves; w++)
+                    o += *(const floatx4 *)(reduce + (w * kRows + r) * kReducePitch + (i & 7) * 4);
+                const bool odd = !finite(o[0]) || !finite(o[1]) || !finite(o[2]) || !finite(o[3]);
+                if (EXACT ? odd || !(sum > 0.0f && finite(sum)) : odd && finite(sum)) again[r] = any_again = 1;
+                const RowAt at = row_at(c, u.row0 + r, h);
+                if (u.part == kNoPart) {
+                    if (d == 0 && !EXACT && !(sum > 0.0f)) *c.bad.word = c.bad.mark;
+                    store_four(c.out, c.out_type, at.token * c.out_stride + (uint64_t)at.head * hd + d, o / sum);
+                } else {
+                    const uint64_t slot = (uint64_t)(u.part + r) * kvh + h;
+                    if (d == 0) c.part_ml[slot] = float2{top - kLift, sum};
+                    *(f32x4a4 *)(c.part_o + slot * hd + d) = o;
+                }
+            }
+        }
+        __syncthreads();
+        if (any_again) careful_rows<BF>(c, u, h, kSplitWaves, again);
+        __syncthreads();
+    }
+}
+
+// Rows whose positions were shared out: one wave a row and KV head.
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnCall c) {
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t hd = c.kv.head_dim, kvh = c.kv.kv_heads;
+    const PlanHeader &head = head_of(c);
+    const JoinItem *items = (const JoinItem *)(c.plan + head.join_at);
+    const uint32_t *parts = (const uint32_t *)(c.plan + head.part_at);
+    const uint32_t total = head.join_count * kvh;
+    for (uint32_t job = blockIdx.x; job < total; job += gridDim.x) {
+        const uint32_t h = job % kvh;
+        const JoinItem it = items[job / kvh];
+        for (uint32_t r = it.row0 + wave; r < it.row0 + it.rows; r += 4) {
+            float top = -INFINITY;
+            for (uint32_t i = 0; i < it.count; i++)
+                top = fmaxf(top, c.part_ml[(uint64_t)(parts[it.first + i] + r) * kvh + h].x);
+            float sum = 0.0f;
+            float o[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[e] = 0.0f;
+            for (uint32_t i = 0; i < it.count; i++) {
+                const uint64_t slot = (uint64_t)(parts[it.first + i] + r) * kvh + h;
+                const float2 ml = c.part_ml[slot];
+                if (ml.y == 0.0f) continue;  // saw nothing
+                const float f = ml.x == top ? 1.0f : exp2_hw(ml.x - top);
+                sum += ml.y * f;
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e++) {
+                    const uint32_t d = e * 64 + lane;
+                    if (d < hd) o[e] = __builtin_fmaf(f, c.part_o[slot * hd + d], o[e]);
+                }
+            }
+            const RowAt at = row_at(c, r, h);
+            if (lane == 0 && !(sum > 0.0f)) *c.bad.word = c.bad.mark;
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) {
+                const uint32_t d = e * 64 + lane;
+                if (d < hd) store_one(c.out, c.out_type, at.token * c.out_stride + (uint64_t)at.head * hd + d, o[e] / sum);
+            }
+        }
+    }
+}
+
+static constexpr int some_blocks(int d) { return d <= 128 ? 4 : 2; }
+
+uint32_t attn_pages_rows(uint32_t cls, uint32_t head_dim, bool exact) {
+    if (cls == 0) return 16;
+    if (cls == 1 && head_dim <= 256) return 16 * some_blocks(head_dim <= 128 ? 128 : 256);
+    return 0;
+}
+
+template <bool BF, int D, bool EXACT>
+static hipError_t launch_split(hipStream_t s, uint32_t cls, uint32_t grid, const AttnCall &call) {
+    if (cls == 0)
+        attn_split_kernel<BF, D, 1, EXACT><<<grid, 64 * kSplitWaves, 0, s>>>(call, cls);
+    else if constexpr (D <= 256)
+        attn_split_kernel<BF, D, some_blocks(D), EXACT><<<grid, 64 * kSplitWaves, 0, s>>>(call, cls);
+    return hipGetLastError();
+}
+
+template <bool BF, bool EXACT>
+static hipError_t launch_dim(hipStream_t s, uint32_t cls, uint32_t grid, const AttnCall &call) {
+    const uint32_t hd = call.kv.head_dim;
+    if (hd <= 64) return launch_split<BF, 64, EXACT>(s, cls, grid, call);
+    if (hd <= 128) return launch_split<BF, 128, EXACT>(s, cls, grid, call);
+    if (hd <= 256) return launch_split<BF, 256, EXACT>(s, cls, grid, call);
+    return launch_split<BF, 512, EXACT>(s, cls, grid, call);
+}
+
+hipError_t launch_attn_pages(hipStream_t s, uint32_t cls, bool bf16, bool exact, uint32_t grid, const AttnCall &call) {
+    if (bf16) return exact ? launch_dim<true, true>(s, cls, grid, call) : launch_dim<true, false>(s, cls, grid, call);
+    return exact ? launch_dim<false, true>(s, cls, grid, call) : launch_dim<false, false>(s, cls, grid, call);
+}
+
+hipError_t launch_attn_join(hipStream_t s, uint32_t grid, const AttnCall &call) {
+    attn_join_kernel<<<grid, 256, 0, s>>>(call);
+    return hipGetLastError();
+}
+
+const void *module_anchor_attn_pages() { return (const void *)attn_join_kernel; }
+
+}  // namespace dm

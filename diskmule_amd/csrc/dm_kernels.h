@@ -56,6 +56,8 @@ hipError_t launch_dense_gemv(hipStream_t s, int cus, uint32_t type, const void *
 const void *module_anchor_expert();
 const void *module_anchor_attention();
 const void *module_anchor_safetensor();
+const void *module_anchor_kv_pages();
+const void *module_anchor_attn_pages();
 
 // GLM safetensors GEMV formats (kernels_safetensor.hip).
 constexpr uint32_t kStBf16 = 0, kStF8 = 1, kStI8 = 2, kStI4 = 3;

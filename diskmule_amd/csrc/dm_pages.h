@@ -1,0 +1,592 @@
+// dm_pages.h -- bookkeeping of a paged KV cache and the work lists of its
+// attention calls.  Plain C++ without any HIP, so that a CPU program can
+// check both over whole ranges of sizes.
+#pragma once
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <functional>
+#include <utility>
+#include <vector>
+
+namespace dm {
+
+constexpr uint32_t kPageTokens = 64;
+constexpr uint32_t kNoPart = 0xffffffffu;
+// Sequences of more query rows than this read what they share each for itself:
+// their own units are as large as a shared one would be.
+constexpr uint32_t kSharedRows = 64;
+
+// An entry of the table updates a call makes: `count` table words from `at`
+// on become page, page + 1, ... or, with kTableCopy set in `value`, copies of
+// the words from (value & ~kTableCopy) on.
+constexpr uint32_t kTableCopy = 0x80000000u;
+struct TableRun {
+    uint32_t at, value, count;
+};
+struct PagePair {
+    uint32_t src, dst;
+};
+// The device work a bookkeeping call asks for, in this order: page copies,
+// then table updates.
+struct PageWork {
+    std::vector<PagePair> copies;
+    std::vector<TableRun> tables;
+    void clear() {
+        copies.clear();
+        tables.clear();
+    }
+};
+
+// Which pages each sequence holds, and how many sequences hold each page.
+// Every operation checks first and changes nothing when it is refused; the
+// lowest free page is always taken first.
+class PageBook {
+   public:
+    struct Sequence {
+        bool live = false;
+        uint64_t length = 0;
+        uint64_t version = 0;  // of the last change, unique over the book's life
+        std::vector<uint32_t> table;
+    };
+    enum class Result { kOk, kNoSequence, kBadSequence, kRepeated, kContext, kNoPages, kLength };
+    // What a refused call names (kContext: position and limit; kNoPages: the
+    // pages that are missing).
+    uint64_t refused_position = 0, refused_limit = 0, refused_pages = 0;
+
+    PageBook(uint32_t pages, uint32_t sequences, uint64_t max_context)
+        : max_context_(max_context), row_((uint32_t)((max_context + kPageTokens - 1) / kPageTokens)) {
+        refs_.assign(pages, 0);
+        marks_.assign(sequences, 0);
+        seqs_.resize(sequences);
+        free_.resize(pages);
+        for (uint32_t i = 0; i < pages; i++) free_[i] = i;  // ascending: a min-heap already
+    }
+
+    uint32_t pages() const { return (uint32_t)refs_.size(); }
+    uint32_t used_pages() const { return pages() - (uint32_t)free_.size(); }
+    uint32_t row() const { return row_; }
+    uint32_t sequences() const { return (uint32_t)seqs_.size(); }
+    uint32_t refs(uint32_t page) const { return refs_[page]; }
+    bool live(size_t s) const { return s < seqs_.size() && seqs_[s].live; }
+    const Sequence &at(size_t s) const { return seqs_[s]; }
+
+    Result create(size_t *out) {
+        for (size_t s = 0; s < seqs_.size(); s++)
+            if (!seqs_[s].live) {
+                open(s);
+                *out = s;
+                return Result::kOk;
+            }
+        return Result::kNoSequence;
+    }
+
+    // `count` tokens more for each sequence; a shared last page that is not
+    // full is copied first, so that the new tokens go to a page of its own.
+    Result extend(size_t n, const size_t *seqs, const size_t *counts, PageWork *work) {
+        if (const Result r = distinct(n, seqs); r != Result::kOk) return r;
+        uint64_t need = 0;
+        for (size_t i = 0; i < n; i++) {
+            const Sequence &s = seqs_[seqs[i]];
+            if (counts[i] > max_context_ - s.length) {
+                refused_position = s.length + std::min<uint64_t>(counts[i], UINT64_MAX - s.length);
+                refused_limit = max_context_;
+                return Result::kContext;
+            }
+            if (counts[i]) need += pages_of(s.length + counts[i]) - s.table.size() + copies_last(s);
+        }
+        if (need > free_.size()) {
+            refused_pages = need - free_.size();
+            return Result::kNoPages;
+        }
+        work->clear();
+        work->tables.reserve((size_t)need);
+        work->copies.reserve(n);
+        for (size_t i = 0; i < n; i++) seqs_[seqs[i]].table.reserve((size_t)pages_of(seqs_[seqs[i]].length + counts[i]));
+        for (size_t i = 0; i < n; i++) {
+            if (!counts[i]) continue;
+            Sequence &s = seqs_[seqs[i]];
+            if (copies_last(s)) {
+                const uint32_t page = take(), old = s.table.back();
+                refs_[old]--;
+                s.table.back() = page;
+                work->copies.push_back({old, page});
+                add_run(work, word(seqs[i], s.table.size() - 1), page);
+            }
+            const uint64_t want = pages_of(s.length + counts[i]);
+            while (s.table.size() < want) {
+                const uint32_t page = take();
+                s.table.push_back(page);
+                add_run(work, word(seqs[i], s.table.size() - 1), page);
+            }
+            s.length += counts[i];
+            s.version = ++clock_;
+        }
+        return Result::kOk;
+    }
+
+    // New sequences holding the first `lengths[i]` tokens of `parents[i]`:
+    // whole pages are shared, a last page that is not full is copied.  A
+    // parent may be named several times.
+    Result fork(size_t n, const size_t *parents, const size_t *lengths, size_t *children, PageWork *work) {
+        uint64_t need = 0;
+        for (size_t i = 0; i < n; i++) {
+            if (!live(parents[i])) return Result::kBadSequence;
+            if (lengths[i] > seqs_[parents[i]].length) {
+                refused_position = lengths[i];
+                refused_limit = seqs_[parents[i]].length;
+                return Result::kLength;
+            }
+            need += lengths[i] % kPageTokens != 0;
+        }
+        size_t found = 0;
+        for (size_t s = 0; s < seqs_.size() && found < n; s++)
+            if (!seqs_[s].live) children[found++] = s;
+        if (found < n) return Result::kNoSequence;
+        if (need > free_.size()) {
+            refused_pages = need - free_.size();
+            return Result::kNoPages;
+        }
+        work->clear();
+        work->copies.reserve((size_t)need);
+        work->tables.reserve(2 * n);
+        for (size_t i = 0; i < n; i++) seqs_[children[i]].table.reserve((size_t)pages_of(lengths[i]));
+        for (size_t i = 0; i < n; i++) {
+            Sequence &parent = seqs_[parents[i]];
+            // its pages become shared: a plan that may write to them is set anew
+            parent.version = ++clock_;
+            Sequence &c = open(children[i]);
+            c.length = lengths[i];
+            const uint32_t whole = (uint32_t)(lengths[i] / kPageTokens);
+            c.table.assign(parent.table.begin(), parent.table.begin() + whole);
+            for (const uint32_t p : c.table) refs_[p]++;
+            if (whole) work->tables.push_back({word(children[i], 0), word(parents[i], 0) | kTableCopy, whole});
+            if (lengths[i] % kPageTokens) {
+                const uint32_t page = take();
+                c.table.push_back(page);
+                work->copies.push_back({parent.table[whole], page});
+                work->tables.push_back({word(children[i], whole), page, 1});
+            }
+        }
+        return Result::kOk;
+    }
+
+    // Tokens past `length` are dropped (a longer length changes nothing).
+    Result truncate(size_t seq, uint64_t length) {
+        if (!live(seq)) return Result::kBadSequence;
+        Sequence &s = seqs_[seq];
+        if (length >= s.length) return Result::kOk;
+        while (s.table.size() > pages_of(length)) {
+            drop(s.table.back());
+            s.table.pop_back();
+        }
+        s.length = length;
+        s.version = ++clock_;
+        return Result::kOk;
+    }
+
+    Result release(size_t n, const size_t *seqs) {
+        if (const Result r = distinct(n, seqs); r != Result::kOk) return r;
+        for (size_t i = 0; i < n; i++) {
+            Sequence &s = seqs_[seqs[i]];
+            for (const uint32_t p : s.table) drop(p);
+            s.table.clear();
+            s.length = 0;
+            s.live = false;
+            s.version = ++clock_;
+        }
+        return Result::kOk;
+    }
+
+    // Pages in use become 0 .. used_pages() - 1: those above, in ascending
+    // order, move to the free ones below, in ascending order.  moves->copies
+    // is sorted by both; no page is moved twice.  Shared pages stay shared.
+    void compact(PageWork *moves) {
+        moves->clear();
+        const uint32_t used = used_pages();
+        std::vector<uint32_t> to(pages(), kNoPart);
+        uint32_t hole = 0;
+        std::vector<uint32_t> refs = refs_;
+        for (uint32_t p = used; p < pages(); p++) {
+            if (!refs_[p]) continue;
+            while (refs[hole]) hole++;
+            to[p] = hole;
+            refs[hole] = refs[p];
+            refs[p] = 0;
+            moves->copies.push_back({p, hole});
+        }
+        std::vector<uint32_t> free(pages() - used);
+        for (uint32_t i = 0; i < free.size(); i++) free[i] = used + i;
+        refs_.swap(refs);
+        free_.swap(free);
+        if (moves->copies.empty()) return;
+        for (Sequence &s : seqs_)
+            for (uint32_t &p : s.table)
+                if (to[p] != kNoPart) p = to[p];
+    }
+
+    // Whether every page that holds one of the sequence's last `count` tokens
+    // is its own.
+    bool writable(size_t seq, uint64_t count) const {
+        const Sequence &s = seqs_[seq];
+        for (uint64_t p = (s.length - count) / kPageTokens; count && p < s.table.size(); p++)
+            if (refs_[s.table[p]] != 1) return false;
+        return true;
+    }
+
+    // Whole pages that a and b begin with in common.
+    uint32_t common_pages(size_t a, size_t b) const {
+        const std::vector<uint32_t> &x = seqs_[a].table, &y = seqs_[b].table;
+        const size_t n = std::min(x.size(), y.size());
+        return (uint32_t)(std::mismatch(x.begin(), x.begin() + n, y.begin()).first - x.begin());
+    }
+
+    Result distinct(size_t n, const size_t *seqs) {
+        mark_++;
+        for (size_t i = 0; i < n; i++) {
+            if (!live(seqs[i])) return Result::kBadSequence;
+            if (marks_[seqs[i]] == mark_) return Result::kRepeated;
+            marks_[seqs[i]] = mark_;
+        }
+        return Result::kOk;
+    }
+
+   private:
+    static uint64_t pages_of(uint64_t tokens) { return (tokens + kPageTokens - 1) / kPageTokens; }
+    uint32_t word(size_t seq, size_t index) const { return (uint32_t)(seq * row_ + index); }
+    bool copies_last(const Sequence &s) const { return s.length % kPageTokens != 0 && refs_[s.table.back()] > 1; }
+    Sequence &open(size_t i) {
+        Sequence &s = seqs_[i];
+        s.live = true;
+        s.length = 0;
+        s.version = ++clock_;
+        s.table.clear();
+        return s;
+    }
+    uint32_t take() {
+        std::pop_heap(free_.begin(), free_.end(), std::greater<uint32_t>());
+        const uint32_t p = free_.back();
+        free_.pop_back();
+        refs_[p] = 1;
+        return p;
+    }
+    void drop(uint32_t p) {
+        if (--refs_[p]) return;
+        free_.push_back(p);  // never more than its first size: no allocation
+        std::push_heap(free_.begin(), free_.end(), std::greater<uint32_t>());
+    }
+    void add_run(PageWork *work, uint32_t at, uint32_t page) {
+        if (!work->tables.empty()) {
+            TableRun &r = work->tables.back();
+            if (!(r.value & kTableCopy) && r.at + r.count == at && r.value + r.count == page) {
+                r.count++;
+                return;
+            }
+        }
+        work->tables.push_back({at, page, 1});
+    }
+
+    uint64_t max_context_;
+    uint32_t row_;
+    uint64_t clock_ = 0, mark_ = 0;
+    std::vector<uint32_t> refs_, free_;  // free_: a min-heap
+    std::vector<uint64_t> marks_;
+    std::vector<Sequence> seqs_;
+};
+
+// ---- the work lists of an attention call ----
+// The rows of a call are its query tokens times the `group` query heads that
+// read one KV head: row r is query head r % group of that KV head, of token
+// r / group.  Every list holds for each KV head.
+
+// Positions [kv0, kv1) of sequence `seq`'s pages for rows row0 .. row0 + rows
+// - 1; kv0 is a multiple of the page.  Positions of [full0, full1) are seen by
+// all of these rows.  part: the first row's place among the partial results,
+// or kNoPart: the unit sees all its rows see, and writes their result itself.
+struct AttnUnit {
+    uint32_t row0, rows, seq, kv0, kv1, full0, full1, part;
+};
+// Rows whose result is joined from `count` partial results: that of row r in
+// part i stands at parts[first + i] + r (modulo 2^32).
+struct JoinItem {
+    uint32_t row0, rows, first, count;
+};
+// Tokens token0 .. token0 + count - 1 of the call stand in one page, in slots
+// slot0 .. of table word `word`.
+struct WriteRun {
+    uint32_t token0, count, word, slot0;
+};
+
+// Kernels by the rows a unit may have: few (16), some (`some_rows`), many
+// (`many_rows`; 0 when the call has no such kernel).
+constexpr uint32_t kUnitClasses = 3;
+
+struct PlanShape {
+    uint32_t group = 1, kv_heads = 1;
+    uint64_t window = 0;  // 0: none
+    uint32_t rows_of[kUnitClasses] = {16, 64, 0};
+    uint32_t workgroups[kUnitClasses] = {512, 512, 512};  // wanted of a launch
+    uint32_t least_chunk[kUnitClasses] = {256, 256, 512}; // positions of a unit, at least, where it is split
+    uint32_t share_pages = 2;                             // whole pages in common from which rows share a unit
+    size_t max_parts = 0;                                 // partial rows (per KV head)
+    size_t max_bytes = 0;                                 // of the lists
+};
+
+struct AttnLists {
+    std::vector<uint32_t> positions;  // of each token
+    std::vector<AttnUnit> units[kUnitClasses];
+    std::vector<JoinItem> joins;
+    std::vector<uint32_t> parts;
+    std::vector<WriteRun> writes;
+    size_t part_rows = 0;
+    size_t bytes() const {
+        size_t b = positions.size() * 4 + joins.size() * sizeof(JoinItem) + parts.size() * 4 +
+                   writes.size() * sizeof(WriteRun);
+        for (const auto &u : units) b += u.size() * sizeof(AttnUnit);
+        return b;
+    }
+};
+
+// The lists' largest size without shared or split units, which is what a plan
+// falls back to: units of 16 rows at least, a page's worth of writes, and one
+// partly filled unit and two partly filled pages of each sequence.
+constexpr size_t plan_least_bytes(size_t tokens, size_t group, size_t sequences) {
+    return tokens * 4 + (tokens * group / 16 + sequences) * sizeof(AttnUnit) +
+           (tokens / kPageTokens + 2 * sequences) * sizeof(WriteRun);
+}
+
+class Planner {
+   public:
+    Planner(const PageBook &book, const PlanShape &shape, size_t n, const size_t *seqs, const size_t *counts)
+        : book_(book), shape_(shape) {
+        uint32_t token = 0;
+        for (size_t i = 0; i < n; i++) {
+            if (!counts[i]) continue;
+            const uint64_t length = book.at(seqs[i]).length;
+            items_.push_back({(uint32_t)seqs[i], token, (uint32_t)counts[i], (uint32_t)(length - counts[i])});
+            token += (uint32_t)counts[i];
+        }
+        tokens_ = token;
+    }
+
+    void build(AttnLists *out) {
+        common_.assign(items_.size(), 0);
+        for (size_t i = 0; i + 1 < items_.size(); i++) {
+            // pages that every query of both sequences may see whole
+            const uint32_t most = std::min(items_[i].first, items_[i + 1].first) / kPageTokens;
+            if (std::max(items_[i].count, items_[i + 1].count) > kSharedRows / shape_.group) continue;
+            common_[i] = std::min(most, book_.common_pages(items_[i].seq, items_[i + 1].seq));
+        }
+        // shared and split; then split alone; then neither, which always fits
+        out_ = out;
+        for (int attempt = 0; attempt < 3; attempt++) {
+            if (attempt == 1) common_.assign(items_.size(), 0);
+            plain_ = attempt == 2;
+            *out = AttnLists();
+            if (lists()) return;
+        }
+    }
+
+   private:
+    struct Item {
+        uint32_t seq, token0, count, first;  // first: position of its first query
+    };
+    // Units over one range of positions for the rows of sequences lo .. hi - 1.
+    struct Level {
+        uint32_t row0, rows, seq, cls, tile;
+        uint64_t kv0, kv1;
+        size_t lo, hi;
+        std::vector<std::vector<uint32_t>> parts;  // of each row tile
+    };
+
+    bool lists() {
+        for (const Item &it : items_) {
+            for (uint32_t t = 0; t < it.count; t++) out_->positions.push_back(it.first + t);
+            for (uint32_t t = 0; t < it.count;) {
+                const uint32_t p = it.first + t, slot = p % kPageTokens;
+                const uint32_t c = std::min(it.count - t, kPageTokens - slot);
+                out_->writes.push_back({it.token0 + t, c, it.seq * book_.row() + p / kPageTokens, slot});
+                t += c;
+            }
+        }
+        levels_.clear();
+        paths_.clear();
+        std::vector<size_t> path;
+        split(0, items_.size(), 0, path);
+        // positions that the units of each class go through, which decide how
+        // long one of them may be
+        uint64_t work[kUnitClasses] = {};
+        for (const Level &l : levels_)
+            for (uint32_t r = 0; r < l.rows; r += l.tile) {
+                uint64_t a, b;
+                range(l, r, &a, &b);
+                work[l.cls] += b - a;
+            }
+        for (uint32_t c = 0; c < kUnitClasses; c++) {
+            const uint64_t per = work[c] * shape_.kv_heads / std::max(1u, shape_.workgroups[c]);
+            chunk_[c] = std::max<uint64_t>(shape_.least_chunk[c], (per + kPageTokens - 1) / kPageTokens * kPageTokens);
+        }
+        std::vector<bool> alone(levels_.size(), false);
+        for (const auto &p : paths_) alone[p.back()] = p.size() == 1;
+        for (size_t i = 0; i < levels_.size(); i++)
+            if (!units(&levels_[i], alone[i])) return false;
+        for (const auto &p : paths_)
+            if (!join(p)) return false;
+        for (auto &u : out_->units)  // long ones first, so that none is begun last
+            std::stable_sort(u.begin(), u.end(),
+                             [](const AttnUnit &a, const AttnUnit &b) { return a.kv1 - a.kv0 > b.kv1 - b.kv0; });
+        return plain_ || fits();
+    }
+
+    bool fits() const { return out_->part_rows <= shape_.max_parts && out_->bytes() <= shape_.max_bytes; }
+
+    // Sequences lo .. hi - 1 hold their first `from` pages in common, and those
+    // are dealt with (levels of `path`): units for what follows.  A run of
+    // sequences that begin alike is found by its neighbours' common pages.
+    void split(size_t lo, size_t hi, uint32_t from, std::vector<size_t> &path) {
+        while (lo < hi) {
+            size_t end = lo + 1;
+            uint32_t common = UINT32_MAX;
+            while (!plain_ && end < hi && common_[end - 1] >= from + shape_.share_pages) {
+                common = std::min(common, common_[end - 1]);
+                end++;
+            }
+            if (end == lo + 1) {
+                const Item &it = items_[lo];
+                path.push_back(level(lo, end, (uint64_t)from * kPageTokens, (uint64_t)it.first + it.count));
+                paths_.push_back(path);
+                path.pop_back();
+            } else {
+                path.push_back(level(lo, end, (uint64_t)from * kPageTokens, (uint64_t)common * kPageTokens));
+                split(lo, end, common, path);
+                path.pop_back();
+            }
+            lo = end;
+        }
+    }
+
+    size_t level(size_t lo, size_t hi, uint64_t kv0, uint64_t kv1) {
+        const Item &last = items_[hi - 1];
+        Level l;
+        l.row0 = items_[lo].token0 * shape_.group;
+        l.rows = (last.token0 + last.count) * shape_.group - l.row0;
+        l.seq = items_[lo].seq;
+        // the smallest kernel that takes all rows in one unit, else the largest there is
+        l.cls = 0;
+        while (l.cls + 1 < kUnitClasses && shape_.rows_of[l.cls + 1] && l.rows > shape_.rows_of[l.cls]) l.cls++;
+        l.tile = shape_.rows_of[l.cls];
+        l.kv0 = kv0;
+        l.kv1 = kv1;
+        l.lo = lo;
+        l.hi = hi;
+        levels_.push_back(l);
+        return levels_.size() - 1;
+    }
+
+    uint32_t position(uint32_t row) const { return out_->positions[row / shape_.group]; }
+
+    // Smallest and largest query position of a tile of a level's rows.
+    void bounds(const Level &l, uint32_t r, uint32_t *low, uint32_t *high) const {
+        const uint32_t a = l.row0 + r, b = std::min(l.row0 + l.rows, a + l.tile) - 1;
+        if (l.hi - l.lo == 1) {  // one sequence: ascending
+            *low = position(a);
+            *high = position(b);
+            return;
+        }
+        *low = UINT32_MAX;
+        *high = 0;
+        for (uint32_t t = a / shape_.group; t <= b / shape_.group; t++) {
+            *low = std::min(*low, out_->positions[t]);
+            *high = std::max(*high, out_->positions[t]);
+        }
+    }
+
+    // The positions that rows r .. of a level's tile see within it: [a, b), a
+    // a multiple of the page; empty where the window has passed them all.
+    void range(const Level &l, uint32_t r, uint64_t *a, uint64_t *b) const {
+        uint32_t low, high;
+        bounds(l, r, &low, &high);
+        const uint64_t first = shape_.window && low + 1ull > shape_.window ? low + 1 - shape_.window : 0;
+        *b = std::min<uint64_t>(l.kv1, (uint64_t)high + 1);
+        *a = std::max<uint64_t>(l.kv0, first / kPageTokens * kPageTokens);
+        if (*a > *b) *a = *b;
+    }
+
+    bool units(Level *l, bool alone) {
+        for (uint32_t r = 0; r < l->rows; r += l->tile) {
+            l->parts.emplace_back();
+            const uint32_t rows = std::min(l->tile, l->rows - r);
+            uint64_t a, b;
+            uint32_t low, high;
+            range(*l, r, &a, &b);
+            bounds(*l, r, &low, &high);
+            if (a == b) continue;
+            // even chunks of whole pages
+            const uint64_t pages = (b - a + kPageTokens - 1) / kPageTokens;
+            uint64_t n = plain_ ? 1 : std::min(pages, (b - a + chunk_[l->cls] - 1) / chunk_[l->cls]);
+            const bool direct = alone && n == 1;
+            const uint64_t full0 = shape_.window && high + 1ull > shape_.window ? high + 1 - shape_.window : 0;
+            for (uint64_t i = 0; i < n; i++) {
+                AttnUnit u;
+                u.row0 = l->row0 + r;
+                u.rows = rows;
+                u.seq = l->seq;
+                u.kv0 = (uint32_t)(a + pages * i / n * kPageTokens);
+                u.kv1 = (uint32_t)std::min(b, a + pages * (i + 1) / n * kPageTokens);
+                u.full0 = (uint32_t)full0;
+                u.full1 = low + 1;
+                u.part = kNoPart;
+                if (!direct) {
+                    u.part = (uint32_t)out_->part_rows;
+                    l->parts.back().push_back(u.part - u.row0);
+                    out_->part_rows += rows;
+                }
+                out_->units[l->cls].push_back(u);
+            }
+            if (!plain_ && !fits()) return false;
+        }
+        return true;
+    }
+
+    // The rows of the sequence at the end of `path`, in runs that meet the
+    // same units of every level.
+    bool join(const std::vector<size_t> &path) {
+        const Level &leaf = levels_[path.back()];
+        if (path.size() == 1) {
+            bool any = false;
+            for (const auto &p : leaf.parts) any = any || !p.empty();
+            if (!any) return true;
+        }
+        uint32_t r = leaf.row0;
+        const uint32_t end = leaf.row0 + leaf.rows;
+        while (r < end) {
+            JoinItem item{r, end - r, (uint32_t)out_->parts.size(), 0};
+            for (const size_t i : path) {
+                const Level &l = levels_[i];
+                const uint32_t tile = (r - l.row0) / l.tile;
+                item.rows = std::min(item.rows, l.row0 + (tile + 1) * l.tile - r);
+                for (const uint32_t p : l.parts[tile]) out_->parts.push_back(p);
+            }
+            item.count = (uint32_t)out_->parts.size() - item.first;
+            if (item.count) out_->joins.push_back(item);  // none: the one unit wrote its rows itself
+            r += item.rows;
+            if (!plain_ && !fits()) return false;
+        }
+        return true;
+    }
+
+    const PageBook &book_;
+    PlanShape shape_;
+    std::vector<Item> items_;
+    uint32_t tokens_ = 0;
+    bool plain_ = false;
+    AttnLists *out_ = nullptr;
+    std::vector<uint32_t> common_;  // of item i and item i + 1
+    std::vector<Level> levels_;
+    std::vector<std::vector<size_t>> paths_;
+    uint64_t chunk_[kUnitClasses] = {};
+};
+
+}  // namespace dm

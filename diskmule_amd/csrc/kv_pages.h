@@ -1,0 +1,55 @@
+// kv_pages.h -- the paged KV cache's device side: what its kernels are handed
+// and their launchers.
+#pragma once
+
+#include "dm_kernels.h"
+#include "dm_pages.h"
+
+namespace dm {
+
+// The head of a plan's device copy: how many entries its lists have and where
+// they begin, in bytes from the head.  Kernels read both from here, so that a
+// captured launch works on whatever the plan holds when it is replayed.
+struct PlanHeader {
+    uint32_t unit_count[kUnitClasses];
+    uint32_t join_count, write_count, token_count;
+    uint32_t unit_at[kUnitClasses];
+    uint32_t position_at, join_at, part_at, write_at;
+    uint32_t pad[3];
+};
+static_assert(sizeof(PlanHeader) == 64, "the lists behind the head stay 16-byte aligned");
+
+// One layer's pages.  A page holds a block for each KV head: its 64 keys as
+// [head_dim / 8][64][8], then its 64 values as [8][head_dim][8], element j of
+// chunk c being token 16 (c / 2) + 4 (c % 2) + 8 (j / 4) + j % 4 of the page.
+// Both are the order in which the matrix instructions' operands read them, 16
+// bytes a lane: eight dims of one key, and eight values of one dim whose
+// tokens are the ones of which the lane holds the scores.
+struct PagesView {
+    void *base;             // the layer's first page
+    const uint32_t *table;  // [sequences][row] page numbers
+    uint32_t row, kv_heads, head_dim;
+};
+
+struct AttnCall {
+    PagesView kv;
+    const uint8_t *plan;  // PlanHeader and its lists
+    const void *q;
+    void *out;
+    uint64_t q_stride, out_stride;  // elements from one token's row to the next
+    uint32_t q_type, out_type;      // ggml ids
+    uint32_t group, window;         // window 0: none
+    float scale;                    // of a score, times log2(e)
+    float *part_o;                  // [row][kv_heads][head_dim]
+    float2 *part_ml;                // [row][kv_heads]: largest scaled score, sum
+    BadFlag bad;
+};
+
+// Rows of a unit of each class for a head dimension; many is 0 where the
+// exact kernels (32-bit outputs) run.
+uint32_t attn_pages_rows(uint32_t cls, uint32_t head_dim, bool exact);
+// Enqueues the units of `cls` on `grid` workgroups of a pool of F16 or BF16.
+hipError_t launch_attn_pages(hipStream_t s, uint32_t cls, bool bf16, bool exact, uint32_t grid, const AttnCall &call);
+hipError_t launch_attn_join(hipStream_t s, uint32_t grid, const AttnCall &call);
+
+}  // namespace dm

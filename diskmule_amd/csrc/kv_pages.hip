@@ -1,0 +1,698 @@
+// kv_pages.hip -- the paged KV cache: its memory and tables, the kernels that
+// write, copy and move pages, and the entry points of cache and attention.
+//
+// Bookkeeping (dm_pages.h) is on the host and current when a call returns;
+// the device's copy of the tables follows on the context's stream, by kernels
+// that carry what changed in their arguments, so that no call waits and no
+// host memory has to outlive one.
+#include <math.h>
+#include <string.h>
+
+#include <new>
+
+#include "dm_device.h"
+#include "kv_pages.h"
+#include "runtime.h"
+
+namespace dm {
+
+typedef uint32_t u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// Kernel arguments hold 4 KiB.
+constexpr uint32_t kRunsPerLaunch = 320, kPairsPerLaunch = 480;
+struct TableRuns {
+    TableRun run[kRunsPerLaunch];
+};
+struct PagePairs {
+    PagePair pair[kPairsPerLaunch];
+};
+
+__global__ __launch_bounds__(64) void table_runs_kernel(uint32_t *table, TableRuns runs) {
+    const TableRun r = runs.run[blockIdx.x];
+    for (uint32_t i = threadIdx.x; i < r.count; i += 64)
+        table[r.at + i] = r.value & kTableCopy ? table[(r.value & ~kTableCopy) + i] : r.value + i;
+}
+
+// Table words that name a moved page name its new place: pairs ascend in src.
+__global__ __launch_bounds__(256) void table_moves_kernel(uint32_t *table, uint32_t words, PagePairs pairs,
+                                                          uint32_t count) {
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (uint64_t)gridDim.x * 256) {
+        const uint32_t page = table[i];
+        uint32_t lo = 0, hi = count;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (pairs.pair[mid].src < page)
+                lo = mid + 1;
+            else
+                hi = mid;
+        }
+        if (lo < count && pairs.pair[lo].src == page) table[i] = pairs.pair[lo].dst;
+    }
+}
+
+// Whole pages of every layer: 16 KiB a workgroup, four 16-byte loads of a
+// thread in flight.  Bound by memory.
+constexpr uint32_t kCopyBytes = 16384;
+__global__ __launch_bounds__(256) void copy_pages_kernel(uint8_t *base, uint64_t layer_bytes, uint32_t page_bytes,
+                                                         PagePairs pairs) {
+    const PagePair p = pairs.pair[blockIdx.y];
+    uint8_t *layer = base + blockIdx.z * layer_bytes;
+    const uint8_t *src = layer + (uint64_t)p.src * page_bytes;
+    uint8_t *dst = layer + (uint64_t)p.dst * page_bytes;
+    const uint32_t at = blockIdx.x * kCopyBytes + threadIdx.x * 16;
+    u32x4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (at + i * 4096 < page_bytes) v[i] = *(const u32x4 *)(src + at + i * 4096);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (at + i * 4096 < page_bytes) *(u32x4 *)(dst + at + i * 4096) = v[i];
+}
+
+struct WriteCall {
+    PagesView kv;
+    const uint8_t *plan;
+    const void *rows[2];  // keys, values
+    uint64_t stride[2];
+    uint32_t source_type;
+};
+
+// Rows of keys (z = 0) or values (z = 1) into pages: a workgroup takes one
+// run of a page for one head, 32 slots at a time through LDS, so that rows are
+// read and pages written 16 bytes a lane.  Value chunks of which the run
+// holds only some tokens are written a value at a time.  Bound by memory.
+template <typename T>
+__global__ __launch_bounds__(256) void write_pages_kernel(WriteCall c) {
+    extern __shared__ __attribute__((aligned(16))) uint16_t tile[];  // [32][head_dim + 8]
+    const PlanHeader &head = *(const PlanHeader *)c.plan;
+    const WriteRun *runs = (const WriteRun *)(c.plan + head.write_at);
+    const uint32_t hd = c.kv.head_dim, h = blockIdx.y, values = blockIdx.z, pitch = hd + 8, eights = hd / 8;
+    const void *rows = c.rows[values];
+    const uint64_t stride = c.stride[values];
+    for (uint32_t i = blockIdx.x; i < head.write_count; i += gridDim.x) {
+        const WriteRun r = runs[i];
+        const uint32_t page = c.kv.table[r.word];
+        T *block = (T *)c.kv.base + ((uint64_t)page * c.kv.kv_heads + h) * 2 * hd * kPageTokens + values * hd * kPageTokens;
+        for (uint32_t s0 = r.slot0 & ~31u; s0 < r.slot0 + r.count; s0 += 32) {
+            const uint32_t a = r.slot0 > s0 ? r.slot0 - s0 : 0, b = min(32u, r.slot0 + r.count - s0);
+            for (uint32_t w = threadIdx.x; w < (b - a) * eights; w += 256) {
+                const uint32_t slot = a + w / eights, ch = w % eights;
+                const uint64_t at = (uint64_t)(r.token0 + s0 + slot - r.slot0) * stride + (uint64_t)h * hd + ch * 8;
+                u32x4 out;
+                if (c.source_type == kF32) {
+                    const f32x4a4 x = *(const f32x4a4 *)((const float *)rows + at);
+                    const f32x4a4 y = *(const f32x4a4 *)((const float *)rows + at + 4);
+                    typedef T t8 __attribute__((ext_vector_type(8)));
+                    const t8 v = {(T)x[0], (T)x[1], (T)x[2], (T)x[3], (T)y[0], (T)y[1], (T)y[2], (T)y[3]};
+                    out = __builtin_bit_cast(u32x4, v);
+                } else {
+                    out = *(const u32x4a2 *)((const uint16_t *)rows + at);
+                }
+                *(u32x4 *)(tile + slot * pitch + ch * 8) = out;
+            }
+            __syncthreads();
+            if (!values) {
+                for (uint32_t w = threadIdx.x; w < 32 * eights; w += 256) {
+                    const uint32_t slot = w & 31, ch = w >> 5;
+                    if (slot >= a && slot < b)
+                        *(u32x4 *)((uint16_t *)block + (ch * kPageTokens + s0 + slot) * 8) =
+                            *(const u32x4 *)(tile + slot * pitch + ch * 8);
+                }
+            } else {
+                for (uint32_t w = threadIdx.x; w < 4 * hd; w += 256) {
+                    const uint32_t chunk = w / hd, d = w % hd;
+                    const uint32_t t0 = 16 * (chunk >> 1) + 4 * (chunk & 1);  // tokens t0 .. + 3, t0 + 8 .. + 11
+                    uint16_t *dst = (uint16_t *)block + ((uint64_t)((s0 / 8 + chunk) * hd + d)) * 8;
+                    if (a <= t0 && b >= t0 + 12) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (uint32_t j = 0; j < 4; j++) {
+                            const uint32_t t = t0 + 2 * (j & 1) + 8 * (j >> 1);
+                            v[j] = (uint32_t)tile[t * pitch + d] | ((uint32_t)tile[(t + 1) * pitch + d] << 16);
+                        }
+                        *(u32x4 *)dst = u32x4{v[0], v[1], v[2], v[3]};
+                    } else {
+#pragma unroll
+                        for (uint32_t j = 0; j < 8; j++) {
+                            const uint32_t t = t0 + (j & 3) + 8 * (j >> 2);
+                            if (t >= a && t < b) dst[j] = tile[t * pitch + d];
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+        }
+    }
+}
+
+const void *module_anchor_kv_pages() { return (const void *)table_runs_kernel; }
+
+}  // namespace dm
+
+using namespace dm;
+
+struct dmhip_kv_pages {
+    dmhip_ctx *ctx = nullptr;
+    int device = 0;
+    uint32_t type = 0;
+    uint32_t layers = 0, kv_heads = 0, head_dim = 0;
+    uint32_t page_bytes = 0;
+    uint64_t layer_bytes = 0;
+    uint8_t *data = nullptr;
+    uint32_t *table = nullptr;
+    size_t plans = 0;     // that refer to this
+    bool closed = false;  // freed by its owner; its plans refuse every call
+    PageBook book;
+    PageWork work;
+    dmhip_kv_pages(uint32_t pages, uint32_t sequences, uint64_t max_context) : book(pages, sequences, max_context) {}
+    PagesView view(uint32_t layer) const {
+        return {data + layer * layer_bytes, table, book.row(), kv_heads, head_dim};
+    }
+};
+
+struct dmhip_kv_plan {
+    static constexpr int kRing = 4;  // settings whose copies may be in flight
+    dmhip_kv_pages *pool = nullptr;
+    uint32_t query_heads = 0, query_type = 0, output_type = 0;
+    size_t max_tokens = 0;
+    PlanShape shape;
+    size_t list_bytes = 0;
+    uint8_t *lists = nullptr;  // device: PlanHeader and lists
+    uint8_t *staging[kRing] = {};
+    hipEvent_t copied[kRing] = {};
+    int next = 0;
+    float *part_o = nullptr;
+    float2 *part_ml = nullptr;
+    PlanHeader head{};
+    bool set = false;
+    bool writable = false;
+    struct Of {
+        size_t seq;
+        uint64_t version;
+    };
+    std::vector<Of> of;  // the sequences as they were set
+    AttnLists build;
+};
+
+namespace dm {
+
+static int fail_overflow() { return fail(DMHIP_ERR_OVERFLOW, "matrix dimensions or encoded byte length overflowed"); }
+
+static int refuse(const dmhip_kv_pages *pool, PageBook::Result r) {
+    switch (r) {
+    case PageBook::Result::kOk: return DMHIP_OK;
+    case PageBook::Result::kNoSequence:
+        return fail(DMHIP_ERR_NO_SLOTS, "all %u sequences of the paged KV cache are in use", pool->book.sequences());
+    case PageBook::Result::kBadSequence: return fail(DMHIP_ERR_INVALID_ARGUMENT, "no such sequence in the paged KV cache");
+    case PageBook::Result::kRepeated: return fail(DMHIP_ERR_INVALID_ARGUMENT, "a sequence is named twice in one call");
+    case PageBook::Result::kContext:
+    case PageBook::Result::kLength:
+        return fail_kv_context((size_t)pool->book.refused_position, (size_t)pool->book.refused_limit);
+    case PageBook::Result::kNoPages:
+        return fail_alloc((size_t)pool->book.refused_pages * pool->page_bytes * pool->layers);
+    }
+    return fail(DMHIP_ERR_INVALID_ARGUMENT, "paged KV cache");
+}
+
+// Calls that change the tables, or copy from host memory, are no work that a
+// graph could replay.
+static int refuse_capture(dmhip_ctx *ctx, const char *what) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    DM_HIP(hipStreamIsCapturing(ctx->stream, &st));
+    if (st != hipStreamCaptureStatusNone)
+        return fail(DMHIP_ERR_INVALID_ARGUMENT, "%s cannot be captured into a graph", what);
+    return DMHIP_OK;
+}
+
+static int enqueue_copies(dmhip_kv_pages *p) {
+    const std::vector<PagePair> &copies = p->work.copies;
+    for (size_t i = 0; i < copies.size(); i += kPairsPerLaunch) {
+        const uint32_t n = (uint32_t)std::min<size_t>(kPairsPerLaunch, copies.size() - i);
+        PagePairs args;
+        memcpy(args.pair, copies.data() + i, n * sizeof(PagePair));
+        for (uint32_t layer = 0; layer < p->layers; layer += 32768) {
+            const uint32_t layers = std::min(p->layers - layer, 32768u);
+            copy_pages_kernel<<<dim3((p->page_bytes + kCopyBytes - 1) / kCopyBytes, n, layers), 256, 0, p->ctx->stream>>>(
+                p->data + layer * p->layer_bytes, p->layer_bytes, p->page_bytes, args);
+            DM_HIP(hipGetLastError());
+        }
+    }
+    return DMHIP_OK;
+}
+
+static int enqueue_tables(dmhip_kv_pages *p) {
+    const std::vector<TableRun> &runs = p->work.tables;
+    for (size_t i = 0; i < runs.size(); i += kRunsPerLaunch) {
+        const uint32_t n = (uint32_t)std::min<size_t>(kRunsPerLaunch, runs.size() - i);
+        TableRuns args;
+        memcpy(args.run, runs.data() + i, n * sizeof(TableRun));
+        table_runs_kernel<<<n, 64, 0, p->ctx->stream>>>(p->table, args);
+        DM_HIP(hipGetLastError());
+    }
+    return DMHIP_OK;
+}
+
+static int enqueue_moves(dmhip_kv_pages *p) {
+    const std::vector<PagePair> &moves = p->work.copies;
+    const uint32_t words = p->book.sequences() * p->book.row();
+    for (size_t i = 0; i < moves.size(); i += kPairsPerLaunch) {
+        const uint32_t n = (uint32_t)std::min<size_t>(kPairsPerLaunch, moves.size() - i);
+        PagePairs args;
+        memcpy(args.pair, moves.data() + i, n * sizeof(PagePair));
+        table_moves_kernel<<<std::min((words + 255) / 256, 2048u), 256, 0, p->ctx->stream>>>(p->table, words, args, n);
+        DM_HIP(hipGetLastError());
+    }
+    return DMHIP_OK;
+}
+
+static void plan_release(dmhip_kv_plan *plan) {
+    if (plan->lists) (void)hipFree(plan->lists);
+    if (plan->part_o) (void)hipFree(plan->part_o);
+    if (plan->part_ml) (void)hipFree(plan->part_ml);
+    for (int i = 0; i < dmhip_kv_plan::kRing; i++) {
+        if (plan->staging[i]) (void)hipHostFree(plan->staging[i]);
+        if (plan->copied[i]) (void)hipEventDestroy(plan->copied[i]);
+    }
+    delete plan;
+}
+
+// Lays the lists out behind their head, each 16-byte aligned.
+static size_t pack(const AttnLists &l, uint8_t *to, PlanHeader *head) {
+    size_t at = sizeof(PlanHeader);
+    auto put = [&](const void *src, size_t bytes) {
+        const size_t here = at;
+        if (bytes) memcpy(to + here, src, bytes);
+        at = (here + bytes + 15) & ~(size_t)15;
+        return (uint32_t)here;
+    };
+    *head = PlanHeader{};
+    for (uint32_t c = 0; c < kUnitClasses; c++) {
+        head->unit_count[c] = (uint32_t)l.units[c].size();
+        head->unit_at[c] = put(l.units[c].data(), l.units[c].size() * sizeof(AttnUnit));
+    }
+    head->join_count = (uint32_t)l.joins.size();
+    head->write_count = (uint32_t)l.writes.size();
+    head->token_count = (uint32_t)l.positions.size();
+    head->position_at = put(l.positions.data(), l.positions.size() * 4);
+    head->join_at = put(l.joins.data(), l.joins.size() * sizeof(JoinItem));
+    head->part_at = put(l.parts.data(), l.parts.size() * 4);
+    head->write_at = put(l.writes.data(), l.writes.size() * sizeof(WriteRun));
+    memcpy(to, head, sizeof *head);
+    return at;
+}
+
+static int plan_checks(dmhip_ctx *ctx, const dmhip_kv_plan *plan, size_t layer) {
+    if (plan->pool->closed) return fail(DMHIP_ERR_INVALID_ARGUMENT, "the plan's paged KV cache was freed");
+    if (plan->pool->ctx != ctx) return fail(DMHIP_ERR_INVALID_ARGUMENT, "the plan belongs to another context");
+    if (!plan->set) return fail(DMHIP_ERR_INVALID_ARGUMENT, "the plan was not set");
+    for (const dmhip_kv_plan::Of &o : plan->of)
+        if (plan->pool->book.at(o.seq).version != o.version)
+            return fail(DMHIP_ERR_INVALID_ARGUMENT, "sequence %zu has changed since the plan was set", o.seq);
+    if (layer >= plan->pool->layers) {
+        fail(DMHIP_ERR_INVALID_LAYER, "layer %zu is outside the paged KV cache's %u layers", layer, plan->pool->layers);
+        last_detail().layer = layer;
+        last_detail().count = plan->pool->layers;
+        return DMHIP_ERR_INVALID_LAYER;
+    }
+    return DMHIP_OK;
+}
+
+static size_t type_bytes(uint32_t type) { return type == kF32 ? 4 : 2; }
+
+static int aligned(const void *p, uint32_t type, const char *what) {
+    if ((uintptr_t)p % type_bytes(type))
+        return fail(DMHIP_ERR_INVALID_ARGUMENT, "%s are not aligned to their type", what);
+    return DMHIP_OK;
+}
+
+// Workgroups of a captured launch, which has to serve whatever the plan holds
+// when it is replayed: each goes on to the next unit until there is none.
+static uint32_t captured_grid(const dmhip_ctx *ctx) { return 4u * (ctx->compute_units > 0 ? ctx->compute_units : 256); }
+
+}  // namespace dm
+
+#define DM_REQUIRE_PTR(ptr)                                                              \
+    do {                                                                                 \
+        if (!(ptr)) return fail(DMHIP_ERR_INVALID_ARGUMENT, "%s must not be null", #ptr); \
+    } while (0)
+
+// No exception crosses the boundary: the host's own lists are all that throws.
+#define DM_HOST_MEMORY(statement)                                                                    \
+    try {                                                                                            \
+        statement;                                                                                   \
+    } catch (const std::exception &) {                                                               \
+        return fail(DMHIP_ERR_BUFFER_ALLOCATION, "could not allocate the host lists of the KV pages"); \
+    }
+
+extern "C" {
+
+int dmhip_new_kv_pages(dmhip_ctx *ctx, uint32_t ggml_type, size_t layers, size_t kv_heads, size_t head_dimension,
+                       size_t max_context, size_t pages, size_t sequences, dmhip_kv_pages **out) {
+    DM_REQUIRE_PTR(ctx);
+    DM_REQUIRE_PTR(out);
+    *out = nullptr;
+    if (ggml_type != kF16 && ggml_type != kBF16) return fail_unsupported(ggml_type, "paged KV cache");
+    if (layers == 0 || kv_heads == 0 || max_context == 0 || pages == 0 || sequences == 0)
+        return fail_shape("paged KV cache layers, heads, context, pages and sequences must be non-zero");
+    if (head_dimension == 0 || head_dimension % 8 != 0 || head_dimension > 512)
+        return fail_shape("paged KV cache head dimensions are multiples of 8 up to 512");
+    const size_t row = max_context / kPageTokens + (max_context % kPageTokens != 0);
+    size_t words, bytes;
+    if (__builtin_mul_overflow(row, sequences, &words) || words >= kTableCopy || pages >= kTableCopy ||
+        layers > 0xffffu || kv_heads > 0xffffu || max_context >= kTableCopy)
+        return fail(DMHIP_ERR_VECTOR_TOO_LARGE, "HIP vector length exceeds the 32-bit kernel limit");
+    const size_t page_bytes = kv_heads * 2 * head_dimension * kPageTokens * 2;
+    if (page_bytes > 0x7fffffffu) return fail(DMHIP_ERR_VECTOR_TOO_LARGE, "HIP vector length exceeds the 32-bit kernel limit");
+    if (__builtin_mul_overflow(page_bytes * pages, layers, &bytes) || bytes > SIZE_MAX / 2) return fail_overflow();
+    DM_CHECK_STATUS(set_device(ctx));
+    DM_CHECK_STATUS(refuse_capture(ctx, "making a paged KV cache"));
+    uint8_t *data = nullptr;
+    uint32_t *table = nullptr;
+    if (hipMalloc((void **)&data, bytes) != hipSuccess) {
+        (void)hipGetLastError();
+        return fail_alloc(bytes);
+    }
+    if (hipMalloc((void **)&table, words * 4) != hipSuccess) {
+        (void)hipGetLastError();
+        (void)hipFree(data);
+        return fail_alloc(words * 4);
+    }
+    dmhip_kv_pages *p = nullptr;
+    try {
+        p = new dmhip_kv_pages((uint32_t)pages, (uint32_t)sequences, max_context);
+    } catch (const std::exception &) {
+        (void)hipFree(data);
+        (void)hipFree(table);
+        return fail_alloc(pages * 8);
+    }
+    p->ctx = ctx;
+    p->device = ctx->device;
+    p->type = ggml_type;
+    p->layers = (uint32_t)layers;
+    p->kv_heads = (uint32_t)kv_heads;
+    p->head_dim = (uint32_t)head_dimension;
+    p->page_bytes = (uint32_t)page_bytes;
+    p->layer_bytes = (uint64_t)page_bytes * pages;
+    p->data = data;
+    p->table = table;
+    // zeros, as a new owned buffer holds; and table words that no sequence has
+    // reached yet name a page all the same
+    hipError_t e = hipMemsetAsync(p->data, 0, bytes, ctx->stream);
+    if (e == hipSuccess) e = hipMemsetAsync(p->table, 0, words * 4, ctx->stream);
+    if (e != hipSuccess) {
+        (void)hipFree(p->data);
+        (void)hipFree(p->table);
+        delete p;
+        return hip_fail(e, "clearing the paged KV cache");
+    }
+    *out = p;
+    return DMHIP_OK;
+}
+
+void dmhip_kv_pages_free(dmhip_kv_pages *pool) {
+    if (!pool || pool->closed) return;
+    (void)hipSetDevice(pool->device);
+    // work already enqueued on the context stream may still use the pages
+    if (pool->ctx && pool->ctx->stream) (void)hipStreamSynchronize(pool->ctx->stream);
+    (void)hipFree(pool->data);
+    (void)hipFree(pool->table);
+    pool->data = nullptr;
+    pool->table = nullptr;
+    pool->closed = true;
+    if (pool->plans == 0) delete pool;  // else its last plan does
+}
+
+size_t dmhip_kv_pages_capacity(const dmhip_kv_pages *pool) { return pool ? pool->book.pages() : 0; }
+size_t dmhip_kv_pages_used(const dmhip_kv_pages *pool) { return pool ? pool->book.used_pages() : 0; }
+size_t dmhip_kv_pages_page_bytes(const dmhip_kv_pages *pool) { return pool ? pool->page_bytes : 0; }
+size_t dmhip_kv_pages_allocated_bytes(const dmhip_kv_pages *pool) {
+    return pool ? (size_t)(pool->layer_bytes * pool->layers) : 0;
+}
+void *dmhip_kv_pages_layer(const dmhip_kv_pages *pool, size_t layer) {
+    return pool && !pool->closed && layer < pool->layers ? pool->data + layer * pool->layer_bytes : nullptr;
+}
+
+int dmhip_kv_sequence_new(dmhip_kv_pages *pool, size_t *sequence) {
+    DM_REQUIRE_PTR(pool);
+    DM_REQUIRE_PTR(sequence);
+    return refuse(pool, pool->book.create(sequence));
+}
+
+size_t dmhip_kv_sequence_length(const dmhip_kv_pages *pool, size_t sequence) {
+    return pool && pool->book.live(sequence) ? (size_t)pool->book.at(sequence).length : 0;
+}
+
+int dmhip_kv_sequence_pages(const dmhip_kv_pages *pool, size_t sequence, uint32_t *pages, size_t capacity,
+                            size_t *count) {
+    DM_REQUIRE_PTR(pool);
+    DM_REQUIRE_PTR(count);
+    if (!pool->book.live(sequence)) return refuse(pool, PageBook::Result::kBadSequence);
+    const std::vector<uint32_t> &table = pool->book.at(sequence).table;
+    *count = table.size();
+    const size_t n = std::min(capacity, table.size());
+    if (n == 0) return DMHIP_OK;
+    DM_REQUIRE_PTR(pages);
+    memcpy(pages, table.data(), n * 4);
+    return DMHIP_OK;
+}
+
+int dmhip_kv_sequence_truncate(dmhip_kv_pages *pool, size_t sequence, size_t length) {
+    DM_REQUIRE_PTR(pool);
+    return refuse(pool, pool->book.truncate(sequence, length));
+}
+
+int dmhip_kv_sequences_free(dmhip_kv_pages *pool, size_t count, const size_t *sequences) {
+    DM_REQUIRE_PTR(pool);
+    if (count == 0) return DMHIP_OK;
+    DM_REQUIRE_PTR(sequences);
+    return refuse(pool, pool->book.release(count, sequences));
+}
+
+int dmhip_kv_sequences_extend(dmhip_kv_pages *pool, size_t count, const size_t *sequences, const size_t *tokens) {
+    DM_REQUIRE_PTR(pool);
+    if (count == 0) return DMHIP_OK;
+    DM_REQUIRE_PTR(sequences);
+    DM_REQUIRE_PTR(tokens);
+    DM_CHECK_STATUS(set_device(pool->ctx));
+    DM_CHECK_STATUS(refuse_capture(pool->ctx, "extending KV sequences"));
+    DM_HOST_MEMORY(DM_CHECK_STATUS(refuse(pool, pool->book.extend(count, sequences, tokens, &pool->work))));
+    DM_CHECK_STATUS(enqueue_copies(pool));
+    return enqueue_tables(pool);
+}
+
+int dmhip_kv_sequences_fork(dmhip_kv_pages *pool, size_t count, const size_t *parents, const size_t *lengths,
+                            size_t *children) {
+    DM_REQUIRE_PTR(pool);
+    if (count == 0) return DMHIP_OK;
+    DM_REQUIRE_PTR(parents);
+    DM_REQUIRE_PTR(lengths);
+    DM_REQUIRE_PTR(children);
+    DM_CHECK_STATUS(set_device(pool->ctx));
+    DM_CHECK_STATUS(refuse_capture(pool->ctx, "forking KV sequences"));
+    DM_HOST_MEMORY(DM_CHECK_STATUS(refuse(pool, pool->book.fork(count, parents, lengths, children, &pool->work))));
+    DM_CHECK_STATUS(enqueue_copies(pool));
+    return enqueue_tables(pool);
+}
+
+int dmhip_kv_pages_compact(dmhip_kv_pages *pool, size_t *moved) {
+    DM_REQUIRE_PTR(pool);
+    DM_CHECK_STATUS(set_device(pool->ctx));
+    DM_CHECK_STATUS(refuse_capture(pool->ctx, "compacting KV pages"));
+    DM_HOST_MEMORY(pool->book.compact(&pool->work));
+    if (moved) *moved = pool->work.copies.size();
+    DM_CHECK_STATUS(enqueue_copies(pool));
+    return enqueue_moves(pool);
+}
+
+int dmhip_new_kv_plan(dmhip_kv_pages *pool, size_t query_heads, int has_window, size_t sliding_window,
+                      uint32_t query_type, uint32_t output_type, size_t max_tokens, dmhip_kv_plan **out) {
+    DM_REQUIRE_PTR(pool);
+    DM_REQUIRE_PTR(out);
+    *out = nullptr;
+    if (pool->closed) return fail(DMHIP_ERR_INVALID_ARGUMENT, "the paged KV cache was freed");
+    if (query_heads == 0 || query_heads % pool->kv_heads != 0)
+        return fail_shape("query heads must be a non-zero multiple of KV heads");
+    if (has_window && sliding_window == 0) return fail_empty("attention window");
+    if (query_type != kF32 && query_type != pool->type) return fail_unsupported(query_type, "paged attention queries");
+    if (output_type != kF32 && output_type != kF16 && output_type != kBF16)
+        return fail_unsupported(output_type, "paged attention output");
+    if (max_tokens == 0) return fail_empty("attention plan");
+    const size_t group = query_heads / pool->kv_heads;
+    size_t rows;
+    if (__builtin_mul_overflow(max_tokens, group, &rows) || rows >= 0x40000000u)
+        return fail(DMHIP_ERR_VECTOR_TOO_LARGE, "HIP vector length exceeds the 32-bit kernel limit");
+    DM_CHECK_STATUS(set_device(pool->ctx));
+    DM_CHECK_STATUS(refuse_capture(pool->ctx, "making an attention plan"));
+    dmhip_kv_plan *p = nullptr;
+    DM_HOST_MEMORY(p = new dmhip_kv_plan());
+    p->pool = pool;
+    p->query_heads = (uint32_t)query_heads;
+    p->query_type = query_type;
+    p->output_type = output_type;
+    p->max_tokens = max_tokens;
+    PlanShape &s = p->shape;
+    s.group = (uint32_t)group;
+    s.kv_heads = pool->kv_heads;
+    // a window that holds every position is none
+    s.window = has_window && sliding_window < 0x80000000u ? sliding_window : 0;
+    const uint32_t cus = pool->ctx->compute_units > 0 ? (uint32_t)pool->ctx->compute_units : 256u;
+    uint32_t most = 0;
+    for (uint32_t c = 0; c < kUnitClasses; c++) {
+        s.rows_of[c] = attn_pages_rows(c, pool->head_dim, output_type == kF32);
+        s.workgroups[c] = 2 * cus;
+        most = std::max(most, s.rows_of[c]);
+    }
+    const size_t sequences = std::min<size_t>(pool->book.sequences(), max_tokens);
+    s.max_parts = 2 * std::min(rows, sequences * kSharedRows) + 4 * (size_t)cus * most / pool->kv_heads + most;
+    s.max_bytes = plan_least_bytes(max_tokens, group, sequences) + (512u << 10);
+    p->list_bytes = sizeof(PlanHeader) + s.max_bytes + 16 * 8;
+    const size_t part_rows = s.max_parts * pool->kv_heads;
+    const size_t sizes[3] = {p->list_bytes, part_rows * pool->head_dim * 4, part_rows * sizeof(float2)};
+    void **places[3] = {(void **)&p->lists, (void **)&p->part_o, (void **)&p->part_ml};
+    for (int i = 0; i < 3; i++)
+        if (hipMalloc(places[i], sizes[i]) != hipSuccess) {
+            (void)hipGetLastError();
+            *places[i] = nullptr;
+            plan_release(p);
+            return fail_alloc(sizes[i]);
+        }
+    for (int i = 0; i < dmhip_kv_plan::kRing; i++)
+        if (hipHostMalloc((void **)&p->staging[i], p->list_bytes, hipHostMallocDefault) != hipSuccess ||
+            hipEventCreateWithFlags(&p->copied[i], hipEventDisableTiming) != hipSuccess) {
+            (void)hipGetLastError();
+            plan_release(p);
+            return fail_alloc(p->list_bytes);
+        }
+    pool->plans++;
+    *out = p;
+    return DMHIP_OK;
+}
+
+void dmhip_kv_plan_free(dmhip_kv_plan *plan) {
+    if (!plan) return;
+    dmhip_kv_pages *pool = plan->pool;
+    (void)hipSetDevice(pool->device);
+    // a cache that is closed has waited for its stream, and its context may be gone
+    if (!pool->closed && pool->ctx->stream) (void)hipStreamSynchronize(pool->ctx->stream);
+    plan_release(plan);
+    if (--pool->plans == 0 && pool->closed) delete pool;
+}
+
+int dmhip_kv_plan_set(dmhip_kv_plan *plan, size_t count, const size_t *sequences, const size_t *tokens) {
+    DM_REQUIRE_PTR(plan);
+    DM_REQUIRE_PTR(sequences);
+    DM_REQUIRE_PTR(tokens);
+    dmhip_kv_pages *pool = plan->pool;
+    if (pool->closed) return fail(DMHIP_ERR_INVALID_ARGUMENT, "the plan's paged KV cache was freed");
+    DM_CHECK_STATUS(refuse(pool, pool->book.distinct(count, sequences)));
+    size_t total = 0;
+    bool writable = true;
+    for (size_t i = 0; i < count; i++) {
+        const uint64_t length = pool->book.at(sequences[i]).length;
+        if (tokens[i] > length) return fail_kv_context(tokens[i], (size_t)length);
+        total += tokens[i];
+        writable = writable && pool->book.writable(sequences[i], tokens[i]);
+    }
+    if (total == 0) return fail_empty("attention plan");
+    if (total > plan->max_tokens) return fail_vector_length("attention plan", "tokens", plan->max_tokens, total);
+    DM_CHECK_STATUS(set_device(pool->ctx));
+    DM_CHECK_STATUS(refuse_capture(pool->ctx, "setting an attention plan"));
+    DM_HOST_MEMORY({
+        plan->of.reserve(count);
+        Planner(pool->book, plan->shape, count, sequences, tokens).build(&plan->build);
+    });
+    const int slot = plan->next;
+    DM_HIP(hipEventSynchronize(plan->copied[slot]));  // the setting before the last three has been copied
+    plan->set = false;
+    const size_t bytes = pack(plan->build, plan->staging[slot], &plan->head);
+    DM_HIP(hipMemcpyAsync(plan->lists, plan->staging[slot], bytes, hipMemcpyHostToDevice, pool->ctx->stream));
+    DM_HIP(hipEventRecord(plan->copied[slot], pool->ctx->stream));
+    plan->next = (slot + 1) % dmhip_kv_plan::kRing;
+    plan->of.clear();
+    for (size_t i = 0; i < count; i++)
+        if (tokens[i]) plan->of.push_back({sequences[i], pool->book.at(sequences[i]).version});
+    plan->writable = writable;
+    plan->set = true;
+    return DMHIP_OK;
+}
+
+int dmhip_kv_pages_write_device(dmhip_ctx *ctx, const dmhip_kv_plan *plan, size_t layer, uint32_t source_type,
+                                const void *keys, size_t key_stride, const void *values, size_t value_stride) {
+    DM_REQUIRE_PTR(ctx);
+    DM_REQUIRE_PTR(plan);
+    DM_CHECK_STATUS(plan_checks(ctx, plan, layer));
+    const dmhip_kv_pages *pool = plan->pool;
+    if (source_type != kF32 && source_type != pool->type) return fail_unsupported(source_type, "paged KV cache rows");
+    if (!plan->writable)
+        return fail(DMHIP_ERR_INVALID_ARGUMENT, "tokens of the plan stand in pages that sequences share");
+    const size_t width = (size_t)pool->kv_heads * pool->head_dim;
+    if (key_stride < width) return fail_vector_length("KV pages write", "key stride", width, key_stride);
+    if (value_stride < width) return fail_vector_length("KV pages write", "value stride", width, value_stride);
+    DM_REQUIRE_PTR(keys);
+    DM_REQUIRE_PTR(values);
+    DM_CHECK_STATUS(aligned(keys, source_type, "keys"));
+    DM_CHECK_STATUS(aligned(values, source_type, "values"));
+    DM_CHECK_STATUS(set_device(ctx));
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    DM_HIP(hipStreamIsCapturing(ctx->stream, &st));
+    const uint32_t grid = st == hipStreamCaptureStatusNone ? std::min(plan->head.write_count, 1u << 20) : captured_grid(ctx);
+    const WriteCall call{pool->view((uint32_t)layer), plan->lists, {keys, values}, {key_stride, value_stride}, source_type};
+    const uint32_t lds = 32 * (pool->head_dim + 8) * 2;
+    if (pool->type == kBF16)
+        write_pages_kernel<__bf16><<<dim3(grid, pool->kv_heads, 2), 256, lds, ctx->stream>>>(call);
+    else
+        write_pages_kernel<_Float16><<<dim3(grid, pool->kv_heads, 2), 256, lds, ctx->stream>>>(call);
+    DM_HIP(hipGetLastError());
+    return DMHIP_OK;
+}
+
+int dmhip_attention_pages_device(dmhip_ctx *ctx, const dmhip_kv_plan *plan, size_t layer, float scale,
+                                 const void *query, size_t query_stride, void *output, size_t output_stride) {
+    DM_REQUIRE_PTR(ctx);
+    DM_REQUIRE_PTR(plan);
+    DM_CHECK_STATUS(plan_checks(ctx, plan, layer));
+    const dmhip_kv_pages *pool = plan->pool;
+    if (!isfinite(scale) || scale <= 0.0f) return fail_positive("attention scale");
+    const size_t width = (size_t)plan->query_heads * pool->head_dim;
+    if (query_stride < width) return fail_vector_length("paged attention", "query stride", width, query_stride);
+    if (output_stride < width) return fail_vector_length("paged attention", "output stride", width, output_stride);
+    DM_REQUIRE_PTR(query);
+    DM_REQUIRE_PTR(output);
+    DM_CHECK_STATUS(aligned(query, plan->query_type, "queries"));
+    DM_CHECK_STATUS(aligned(output, plan->output_type, "outputs"));
+    DM_CHECK_STATUS(set_device(ctx));
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    DM_HIP(hipStreamIsCapturing(ctx->stream, &st));
+    const bool captured = st != hipStreamCaptureStatusNone;
+    AttnCall call{};
+    call.kv = pool->view((uint32_t)layer);
+    call.plan = plan->lists;
+    call.q = query;
+    call.out = output;
+    call.q_stride = query_stride;
+    call.out_stride = output_stride;
+    call.q_type = plan->query_type;
+    call.out_type = plan->output_type;
+    call.group = plan->shape.group;
+    call.window = (uint32_t)plan->shape.window;
+    call.scale = scale * 1.44269504088896340736f;
+    call.part_o = plan->part_o;
+    call.part_ml = plan->part_ml;
+    call.bad = attention_device_flag(ctx);
+    const bool exact = plan->output_type == kF32;
+    for (uint32_t c = 0; c < kUnitClasses; c++) {
+        const uint64_t jobs = (uint64_t)plan->head.unit_count[c] * pool->kv_heads;
+        if (!plan->shape.rows_of[c] || (!captured && jobs == 0)) continue;
+        DM_HIP(launch_attn_pages(ctx->stream, c, pool->type == kBF16, exact,
+                                 captured ? captured_grid(ctx) : (uint32_t)std::min<uint64_t>(jobs, 1u << 20), call));
+    }
+    const uint64_t joins = (uint64_t)plan->head.join_count * pool->kv_heads;
+    if (captured || joins)
+        DM_HIP(launch_attn_join(ctx->stream, captured ? captured_grid(ctx) : (uint32_t)std::min<uint64_t>(joins, 1u << 20),
+                                call));
+    ctx->attn_pending = true;
+    return DMHIP_OK;
+}
+
+}  // extern "C"

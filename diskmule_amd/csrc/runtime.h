@@ -37,6 +37,8 @@ int fail_layer(size_t layer, size_t count);
 int fail_expert(size_t layer, size_t expert, size_t count);
 int fail_pinned(size_t layer);
 int fail_io(int os_error);  // 0: unexpected end of file
+int fail_shape(const char *reason);  // InvalidAttentionShape; `reason` static
+int fail_kv_context(size_t position, size_t limit);
 // Maps a HIP runtime error onto DMHIP_ERR_COMMAND (MetalError::Command).
 int hip_fail(hipError_t e, const char *what);
 
@@ -145,6 +147,9 @@ int enqueue_matvec(dmhip_ctx *ctx, uint32_t type, size_t rows, size_t columns, c
 int enqueue_matvec_argmax(dmhip_ctx *ctx, uint32_t type, size_t rows, size_t columns,
                           const void *w, const float *x, float *y, uint32_t *index_device);
 int set_device(dmhip_ctx *ctx);
+// Where a device attention call reports a non-finite score, for
+// dmhip_attention_result.  The caller sets attn_pending once it has enqueued.
+BadFlag attention_device_flag(dmhip_ctx *ctx);
 // Waits until the work enqueued so far on the context's stream is done: the
 // stream writes a sequence number into a pinned word, which the host polls
 // for a while before it falls back to hipStreamSynchronize.

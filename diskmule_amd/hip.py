@@ -57,6 +57,11 @@ EXPORTED_SYMBOLS = [
     "dmhip_matvec_safetensor_mapped", "dmhip_matvec_safetensor", "dmhip_matvec_safetensor_device",
     "dmhip_add", "dmhip_gelu_mul", "dmhip_softmax", "dmhip_rope_neox_in_place", "dmhip_add_device",
     "dmhip_gelu_mul_device", "dmhip_rope_neox_device",
+    "dmhip_new_kv_pages", "dmhip_kv_pages_free", "dmhip_kv_pages_capacity", "dmhip_kv_pages_used",
+    "dmhip_kv_pages_page_bytes", "dmhip_kv_pages_allocated_bytes", "dmhip_kv_pages_layer", "dmhip_kv_sequence_new",
+    "dmhip_kv_sequence_length", "dmhip_kv_sequence_pages", "dmhip_kv_sequence_truncate", "dmhip_kv_sequences_free",
+    "dmhip_kv_sequences_extend", "dmhip_kv_sequences_fork", "dmhip_kv_pages_compact", "dmhip_new_kv_plan",
+    "dmhip_kv_plan_free", "dmhip_kv_plan_set", "dmhip_kv_pages_write_device", "dmhip_attention_pages_device",
 ]
 
 F32, F16, Q5_0, Q8_0, Q4_K, Q6_K, BF16 = 0, 1, 6, 8, 12, 14, 30
@@ -228,6 +233,26 @@ def load_library() -> ctypes.CDLL:
         "dmhip_matvec_safetensor": ([_vp, _u32, _sz, _sz, _u8p, _sz, _f32p, _sz, _f32p, _sz, _f32p, _sz],
                                     ctypes.c_int),
         "dmhip_matvec_safetensor_device": ([_vp, _u32, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp], ctypes.c_int),
+        "dmhip_new_kv_pages": ([_vp, _u32, _sz, _sz, _sz, _sz, _sz, _sz, ctypes.POINTER(_vp)], ctypes.c_int),
+        "dmhip_kv_pages_free": ([_vp], None),
+        "dmhip_kv_pages_capacity": ([_vp], _sz),
+        "dmhip_kv_pages_used": ([_vp], _sz),
+        "dmhip_kv_pages_page_bytes": ([_vp], _sz),
+        "dmhip_kv_pages_allocated_bytes": ([_vp], _sz),
+        "dmhip_kv_pages_layer": ([_vp, _sz], _vp),
+        "dmhip_kv_sequence_new": ([_vp, _szp], ctypes.c_int),
+        "dmhip_kv_sequence_length": ([_vp, _sz], _sz),
+        "dmhip_kv_sequence_pages": ([_vp, _sz, ctypes.POINTER(_u32), _sz, _szp], ctypes.c_int),
+        "dmhip_kv_sequence_truncate": ([_vp, _sz, _sz], ctypes.c_int),
+        "dmhip_kv_sequences_free": ([_vp, _sz, _szp], ctypes.c_int),
+        "dmhip_kv_sequences_extend": ([_vp, _sz, _szp, _szp], ctypes.c_int),
+        "dmhip_kv_sequences_fork": ([_vp, _sz, _szp, _szp, _szp], ctypes.c_int),
+        "dmhip_kv_pages_compact": ([_vp, _szp], ctypes.c_int),
+        "dmhip_new_kv_plan": ([_vp, _sz, ctypes.c_int, _sz, _u32, _u32, _sz, ctypes.POINTER(_vp)], ctypes.c_int),
+        "dmhip_kv_plan_free": ([_vp], None),
+        "dmhip_kv_plan_set": ([_vp, _sz, _szp, _szp], ctypes.c_int),
+        "dmhip_kv_pages_write_device": ([_vp, _vp, _sz, _u32, _vp, _sz, _vp, _sz], ctypes.c_int),
+        "dmhip_attention_pages_device": ([_vp, _vp, _sz, ctypes.c_float, _vp, _sz, _vp, _sz], ctypes.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
@@ -621,6 +646,27 @@ class HipContext:
                                               query_heads, kv_heads, head_dimension, int(window is not None),
                                               window or 0, _fp(output), output.size))
 
+    # -- a paged KV cache, and attention of many sequences over it -------------
+    def new_kv_pages(self, kind: int, layers: int, kv_heads: int, head_dimension: int, max_context: int, pages: int,
+                     sequences: int) -> "KvPages":
+        h = _vp()
+        _check(load_library().dmhip_new_kv_pages(self._h, kind, layers, kv_heads, head_dimension, max_context, pages,
+                                                 sequences, ctypes.byref(h)))
+        return KvPages(self, h.value)
+
+    def write_kv_pages_device(self, plan: "KvPlan", layer: int, source_type: int, k_ptr, k_stride, v_ptr,
+                              v_stride) -> None:
+        """Keys and values of the plan's tokens into their pages of a layer."""
+        _check(load_library().dmhip_kv_pages_write_device(self._h, plan.handle, layer, source_type, k_ptr, k_stride,
+                                                          v_ptr, v_stride))
+
+    def attention_pages_device(self, plan: "KvPlan", layer: int, scale: float, q_ptr, q_stride, out_ptr,
+                               out_stride) -> None:
+        """Causal attention of the plan's tokens over their sequences' pages of
+        a layer; attention_result() reads its non-finite check."""
+        _check(load_library().dmhip_attention_pages_device(self._h, plan.handle, layer, scale, q_ptr, q_stride,
+                                                           out_ptr, out_stride))
+
     # -- routed experts -------------------------------------------------------
     def moe_layer(self, cache: "ExpertCache", layer, batch, hidden, width, experts, k, router_ptr,
                   gate_up_type, down_type, x_ptr, y_ptr):
@@ -672,6 +718,130 @@ class KvLayer:
     def free(self) -> None:
         if getattr(self, "_h", None):
             load_library().dmhip_kv_layer_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def _sizes(values: Sequence[int]):
+    return (_sz * max(len(values), 1))(*values)
+
+
+class KvPages:
+    """A cache of many sequences' keys and values in 64-token pages that
+    sequences may share (include/dmhip.h)."""
+
+    def __init__(self, ctx: HipContext, handle: int):
+        self._ctx = ctx
+        self._h = _vp(handle)
+        ctx._children.add(self)
+
+    @property
+    def handle(self):
+        return self._h
+
+    def page_capacity(self) -> int:
+        return load_library().dmhip_kv_pages_capacity(self._h)
+
+    def used_pages(self) -> int:
+        return load_library().dmhip_kv_pages_used(self._h)
+
+    def page_bytes(self) -> int:
+        return load_library().dmhip_kv_pages_page_bytes(self._h)
+
+    def allocated_bytes(self) -> int:
+        return load_library().dmhip_kv_pages_allocated_bytes(self._h)
+
+    def layer_ptr(self, layer: int) -> int:
+        return load_library().dmhip_kv_pages_layer(self._h, layer) or 0
+
+    def new_sequence(self) -> int:
+        s = _sz()
+        _check(load_library().dmhip_kv_sequence_new(self._h, ctypes.byref(s)))
+        return s.value
+
+    def length(self, sequence: int) -> int:
+        return load_library().dmhip_kv_sequence_length(self._h, sequence)
+
+    def page_ids(self, sequence: int) -> list[int]:
+        n = _sz()
+        _check(load_library().dmhip_kv_sequence_pages(self._h, sequence, None, 0, ctypes.byref(n)))
+        ids = (_u32 * max(n.value, 1))()
+        _check(load_library().dmhip_kv_sequence_pages(self._h, sequence, ids, n.value, ctypes.byref(n)))
+        return list(ids[:n.value])
+
+    def truncate(self, sequence: int, length: int) -> None:
+        _check(load_library().dmhip_kv_sequence_truncate(self._h, sequence, length))
+
+    def release(self, sequences: Sequence[int]) -> None:
+        _check(load_library().dmhip_kv_sequences_free(self._h, len(sequences), _sizes(sequences)))
+
+    def extend(self, sequences: Sequence[int], tokens: Sequence[int]) -> None:
+        if len(sequences) != len(tokens):
+            raise ValueError("extend takes a token count for each sequence")
+        _check(load_library().dmhip_kv_sequences_extend(self._h, len(sequences), _sizes(sequences), _sizes(tokens)))
+
+    def fork(self, parents: Sequence[int], lengths: Sequence[int]) -> list[int]:
+        """New sequences of the first lengths[i] tokens of parents[i]."""
+        if len(parents) != len(lengths):
+            raise ValueError("fork takes a length for each parent")
+        children = _sizes([0] * len(parents))
+        _check(load_library().dmhip_kv_sequences_fork(self._h, len(parents), _sizes(parents), _sizes(lengths),
+                                                      children))
+        return list(children[:len(parents)])
+
+    def compact(self) -> int:
+        """The number of pages moved."""
+        n = _sz()
+        _check(load_library().dmhip_kv_pages_compact(self._h, ctypes.byref(n)))
+        return n.value
+
+    def new_plan(self, query_heads: int, sliding_window: int | None, query_type: int, output_type: int,
+                 max_tokens: int) -> "KvPlan":
+        h = _vp()
+        _check(load_library().dmhip_new_kv_plan(self._h, query_heads, int(sliding_window is not None),
+                                                sliding_window or 0, query_type, output_type, max_tokens,
+                                                ctypes.byref(h)))
+        return KvPlan(self, h.value)
+
+    def free(self) -> None:
+        if getattr(self, "_h", None):
+            load_library().dmhip_kv_pages_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class KvPlan:
+    """The new tokens of a step over a KvPages, and how the work on them is laid
+    out: set once a step, used by every layer."""
+
+    def __init__(self, pages: KvPages, handle: int):
+        self._pages = pages
+        self._h = _vp(handle)
+        pages._ctx._children.add(self)
+
+    @property
+    def handle(self):
+        return self._h
+
+    def set(self, sequences: Sequence[int], tokens: Sequence[int]) -> None:
+        """The last tokens[i] tokens of each sequence are the step's."""
+        if len(sequences) != len(tokens):
+            raise ValueError("set takes a token count for each sequence")
+        _check(load_library().dmhip_kv_plan_set(self._h, len(sequences), _sizes(sequences), _sizes(tokens)))
+
+    def free(self) -> None:
+        if getattr(self, "_h", None):
+            load_library().dmhip_kv_plan_free(self._h)
             self._h = None
 
     def __del__(self):

@@ -134,6 +134,8 @@ typedef struct dmhip_ctx dmhip_ctx;
 typedef struct dmhip_buf dmhip_buf;
 typedef struct dmhip_expert_cache dmhip_expert_cache;
 typedef struct dmhip_kv_layer dmhip_kv_layer;
+typedef struct dmhip_kv_pages dmhip_kv_pages;
+typedef struct dmhip_kv_plan dmhip_kv_plan;
 
 /* ---------------------------------------------------------------------- */
 /* Context, errors, device                                                 */
@@ -494,8 +496,8 @@ int dmhip_attention_cached(dmhip_ctx *ctx, const float *query, size_t query_len,
 int dmhip_attention_cached_device(dmhip_ctx *ctx, const float *query_device, size_t query_len,
                                   const dmhip_kv_layer *layer, size_t query_heads, size_t kv_heads,
                                   size_t head_dimension, float *output_device, size_t output_len);
-/* Waits for the dmhip_attention_cached_device calls made since the previous
-   result (or since a host-slice attention call, which ends that period) and
+/* Waits for the dmhip_attention_cached_device and
+   dmhip_attention_pages_device calls made since the previous result (or since a host-slice attention call, which ends that period) and
    returns NonFinite "softmax" when any of them met a non-finite score (its
    output is then not meaningful).  A host-slice attention call made while
    device calls await their result reports for them too: it returns
@@ -513,6 +515,133 @@ int dmhip_attention(dmhip_ctx *ctx, const float *query, size_t query_len, const 
                     size_t keys_len, const float *values, size_t values_len, size_t query_heads,
                     size_t kv_heads, size_t head_dimension, int has_window, size_t window,
                     float *output, size_t output_len);
+
+/* ---------------------------------------------------------------------- */
+/* A paged KV cache, and attention of many sequences over it               */
+/* ---------------------------------------------------------------------- */
+/* No counterpart in the reference, whose graphs hold one sequence.  A cache
+   holds the keys and values of `sequences` sequences, for `layers` layers of
+   one shape, in pages of 64 tokens that sequences may share.  Which pages a
+   sequence holds is known on the host as soon as a call returns; everything
+   on the device happens in order on the context's stream.  A step of a model:
+
+     dmhip_kv_sequences_extend   each sequence gets room for its new tokens
+     dmhip_kv_plan_set           the new tokens, of which sequences
+     for every layer:
+       dmhip_kv_pages_write_device       the new tokens' keys and values
+       dmhip_attention_pages_device      attention of the new tokens
+
+   The same calls serve a prompt (all its tokens new), a part of one, a decode
+   step (one new token each) and drafted tokens (a few each). */
+
+/* ggml_type: DMHIP_TYPE_F16 or DMHIP_TYPE_BF16, else UnsupportedTensorType.
+   head_dimension: a multiple of 8 up to 512, and none of the sizes zero, else
+   InvalidAttentionShape; a sequence grows to max_context tokens.  VectorTooLarge:
+   max_context or the pages from 2^31, layers or kv_heads from 2^16, sequences
+   times ceil(max_context / 64) from 2^31, or a page from 2^31 bytes.  The pages
+   are zero-filled.  A cache is used from its context's thread. */
+int dmhip_new_kv_pages(dmhip_ctx *ctx, uint32_t ggml_type, size_t layers, size_t kv_heads, size_t head_dimension,
+                       size_t max_context, size_t pages, size_t sequences, dmhip_kv_pages **out);
+/* Waits for the context's stream, then frees the pages.  Call it before
+   dmhip_context_free.  Plans of the cache refuse every call from then on and
+   are freed on their own. */
+void dmhip_kv_pages_free(dmhip_kv_pages *pool);
+/* Pages in all, pages that sequences hold, bytes of a page in one layer, and
+   bytes of all pages of all layers. */
+size_t dmhip_kv_pages_capacity(const dmhip_kv_pages *pool);
+size_t dmhip_kv_pages_used(const dmhip_kv_pages *pool);
+size_t dmhip_kv_pages_page_bytes(const dmhip_kv_pages *pool);
+size_t dmhip_kv_pages_allocated_bytes(const dmhip_kv_pages *pool);
+/* Device address of a layer's pages, the layers one after another: page p
+   begins at p * page_bytes.  It holds, for each KV head, the keys as
+   [head_dimension / 8][64 tokens][8] and then the values as [8 chunks]
+   [head_dimension][8], element j of chunk c being the value of token
+   16 (c / 2) + 4 (c % 2) + 8 (j / 4) + j % 4.  NULL: no such layer. */
+void *dmhip_kv_pages_layer(const dmhip_kv_pages *pool, size_t layer);
+
+/* A new empty sequence: the lowest number not in use; NoSlots when all are. */
+int dmhip_kv_sequence_new(dmhip_kv_pages *pool, size_t *sequence);
+/* Its tokens (0 for a number not in use). */
+size_t dmhip_kv_sequence_length(const dmhip_kv_pages *pool, size_t sequence);
+/* *count: pages that the sequence holds; the first min(capacity, *count) page
+   numbers go to `pages`, which may be NULL for a capacity of 0. */
+int dmhip_kv_sequence_pages(const dmhip_kv_pages *pool, size_t sequence, uint32_t *pages, size_t capacity,
+                            size_t *count);
+/* Drops the tokens from `length` on, as dmhip_kv_layer_truncate does: a longer
+   length changes nothing.  Pages that no sequence holds any more are free. */
+int dmhip_kv_sequence_truncate(dmhip_kv_pages *pool, size_t sequence, size_t length);
+int dmhip_kv_sequences_free(dmhip_kv_pages *pool, size_t count, const size_t *sequences);
+/* Room for tokens[i] more tokens at the end of sequences[i]: the lowest free
+   pages.  The room holds whatever its pages held until it is written.  A shared
+   page that is partly filled is copied first.  KvContext past max_context,
+   BufferAllocation (the bytes missing) when there are not enough pages. */
+int dmhip_kv_sequences_extend(dmhip_kv_pages *pool, size_t count, const size_t *sequences, const size_t *tokens);
+/* New sequences children[i] of the first lengths[i] tokens of parents[i], which
+   may be named several times: whole pages are shared, a last page that is
+   partly filled is copied.  Write the tokens of a parent before it is forked.
+   KvContext: longer than the parent; NoSlots; BufferAllocation. */
+int dmhip_kv_sequences_fork(dmhip_kv_pages *pool, size_t count, const size_t *parents, const size_t *lengths,
+                            size_t *children);
+/* Moves pages so that those in use are 0 .. used - 1, which one copy of each
+   layer saves: the ones above, in ascending order, to the free places below,
+   in ascending order.  Plans stay as they are.  *moved (may be NULL): pages
+   moved. */
+int dmhip_kv_pages_compact(dmhip_kv_pages *pool, size_t *moved);
+/* The calls above check everything before they change anything: a sequence
+   number that is not in use, or is named twice in one call (parents may be),
+   is InvalidArgument.  Those that enqueue work on the device (extend, fork,
+   compact, and making a cache or a plan and setting it) cannot be captured
+   into a graph: InvalidArgument. */
+
+/* What layers of one shape share in a step: which tokens are new, and how the
+   work on them is laid out over the device.  query_heads is a multiple of the
+   cache's kv_heads; with has_window a token sees the last sliding_window
+   tokens up to itself, else all.  query_type: F32 or the cache's type;
+   output_type: F32, F16 or BF16.  With 16-bit output, queries and
+   probabilities are rounded to the cache's type once; with F32 output both
+   are split into two or three such values, which leaves an error of about
+   2^-17 of a probability.  All sums are 32-bit.  Holds device memory for
+   max_tokens tokens a step (and nothing grows later). */
+int dmhip_new_kv_plan(dmhip_kv_pages *pool, size_t query_heads, int has_window, size_t sliding_window,
+                      uint32_t query_type, uint32_t output_type, size_t max_tokens, dmhip_kv_plan **out);
+/* Waits for the context's stream first. */
+void dmhip_kv_plan_free(dmhip_kv_plan *plan);
+/* The step's tokens: the last tokens[i] tokens of each of `count` distinct
+   sequences, packed in this order wherever the calls below take or give rows.
+   Neighbours that begin with the same pages (forks of one parent) read them
+   once for all their tokens, so name such sequences one after another.
+   KvContext: more than a sequence holds; EmptyInput: no token at all;
+   InvalidVectorLength: more than max_tokens.  May wait for the copy of an
+   earlier setting (the fourth before). */
+int dmhip_kv_plan_set(dmhip_kv_plan *plan, size_t count, const size_t *sequences, const size_t *tokens);
+/* Keys and values of the plan's tokens into their pages of a layer: rows of
+   kv_heads * head_dimension values of source_type (F32, rounded to nearest
+   even, or the cache's type), row t at t * stride values; any stride from the
+   row's width, any alignment of the type.  InvalidArgument when the plan was
+   not set, when one of its sequences has changed since (extended, truncated,
+   forked or freed), or when one of its tokens stands in a shared page;
+   InvalidLayer.  Stream-ordered; may be captured. */
+int dmhip_kv_pages_write_device(dmhip_ctx *ctx, const dmhip_kv_plan *plan, size_t layer, uint32_t source_type,
+                                const void *keys, size_t key_stride, const void *values, size_t value_stride);
+/* Causal attention of the plan's tokens over their sequences' pages of a
+   layer: for the token at position p, out = sum_j softmax_j(scale * q . k_j)
+   v_j over the positions j <= p (and j > p - sliding_window); query head h
+   reads KV head h / (query_heads / kv_heads).  Row t of the queries, [query_heads]
+   [head_dimension], stands at t * query_stride values, that of the outputs at
+   t * output_stride; they must not overlap.  Values in positions that a token
+   does not see never reach it, whatever they are.  scale: finite and positive
+   (InvalidPositiveParameter).  A row whose scores hold a NaN or +inf, or only
+   -inf, is reported by dmhip_attention_result (NonFinite "softmax") and not
+   meaningful.  Refusals otherwise as dmhip_kv_pages_write_device.
+
+   Stream-ordered; may be captured.  A captured call works, when it is
+   replayed, on what the plan was last set to, and is not checked against the
+   sequences again: set the plan for each step, and replay on the context's
+   stream or ordered with it.  The plan holds the work space of the call, so
+   calls of one plan must not run at the same time.  dmhip_attention_result
+   reports a replayed call only until the first result after its capture. */
+int dmhip_attention_pages_device(dmhip_ctx *ctx, const dmhip_kv_plan *plan, size_t layer, float scale,
+                                 const void *query, size_t query_stride, void *output, size_t output_stride);
 
 /* ---------------------------------------------------------------------- */
 /* Routed-expert residency (src/expert.rs)                                 */

@@ -60,6 +60,14 @@ pub mod ffi {
     pub struct dmhip_kv_layer {
         _opaque: [u8; 0],
     }
+    #[repr(C)]
+    pub struct dmhip_kv_pages {
+        _opaque: [u8; 0],
+    }
+    #[repr(C)]
+    pub struct dmhip_kv_plan {
+        _opaque: [u8; 0],
+    }
 
     pub const DMHIP_OK: c_int = 0;
     pub const DMHIP_ERR_NO_DEVICE: c_int = 1;
@@ -680,6 +688,95 @@ pub mod ffi {
             window: usize,
             output: *mut f32,
             output_len: usize,
+        ) -> c_int;
+
+        // a paged KV cache, and attention of many sequences over it
+        pub fn dmhip_new_kv_pages(
+            ctx: *mut dmhip_ctx,
+            ggml_type: u32,
+            layers: usize,
+            kv_heads: usize,
+            head_dimension: usize,
+            max_context: usize,
+            pages: usize,
+            sequences: usize,
+            out: *mut *mut dmhip_kv_pages,
+        ) -> c_int;
+        pub fn dmhip_kv_pages_free(pool: *mut dmhip_kv_pages);
+        pub fn dmhip_kv_pages_capacity(pool: *const dmhip_kv_pages) -> usize;
+        pub fn dmhip_kv_pages_used(pool: *const dmhip_kv_pages) -> usize;
+        pub fn dmhip_kv_pages_page_bytes(pool: *const dmhip_kv_pages) -> usize;
+        pub fn dmhip_kv_pages_allocated_bytes(pool: *const dmhip_kv_pages) -> usize;
+        pub fn dmhip_kv_pages_layer(pool: *const dmhip_kv_pages, layer: usize) -> *mut c_void;
+        pub fn dmhip_kv_sequence_new(pool: *mut dmhip_kv_pages, sequence: *mut usize) -> c_int;
+        pub fn dmhip_kv_sequence_length(pool: *const dmhip_kv_pages, sequence: usize) -> usize;
+        pub fn dmhip_kv_sequence_pages(
+            pool: *const dmhip_kv_pages,
+            sequence: usize,
+            pages: *mut u32,
+            capacity: usize,
+            count: *mut usize,
+        ) -> c_int;
+        pub fn dmhip_kv_sequence_truncate(
+            pool: *mut dmhip_kv_pages,
+            sequence: usize,
+            length: usize,
+        ) -> c_int;
+        pub fn dmhip_kv_sequences_free(
+            pool: *mut dmhip_kv_pages,
+            count: usize,
+            sequences: *const usize,
+        ) -> c_int;
+        pub fn dmhip_kv_sequences_extend(
+            pool: *mut dmhip_kv_pages,
+            count: usize,
+            sequences: *const usize,
+            tokens: *const usize,
+        ) -> c_int;
+        pub fn dmhip_kv_sequences_fork(
+            pool: *mut dmhip_kv_pages,
+            count: usize,
+            parents: *const usize,
+            lengths: *const usize,
+            children: *mut usize,
+        ) -> c_int;
+        pub fn dmhip_kv_pages_compact(pool: *mut dmhip_kv_pages, moved: *mut usize) -> c_int;
+        pub fn dmhip_new_kv_plan(
+            pool: *mut dmhip_kv_pages,
+            query_heads: usize,
+            has_window: c_int,
+            sliding_window: usize,
+            query_type: u32,
+            output_type: u32,
+            max_tokens: usize,
+            out: *mut *mut dmhip_kv_plan,
+        ) -> c_int;
+        pub fn dmhip_kv_plan_free(plan: *mut dmhip_kv_plan);
+        pub fn dmhip_kv_plan_set(
+            plan: *mut dmhip_kv_plan,
+            count: usize,
+            sequences: *const usize,
+            tokens: *const usize,
+        ) -> c_int;
+        pub fn dmhip_kv_pages_write_device(
+            ctx: *mut dmhip_ctx,
+            plan: *const dmhip_kv_plan,
+            layer: usize,
+            source_type: u32,
+            keys: *const c_void,
+            key_stride: usize,
+            values: *const c_void,
+            value_stride: usize,
+        ) -> c_int;
+        pub fn dmhip_attention_pages_device(
+            ctx: *mut dmhip_ctx,
+            plan: *const dmhip_kv_plan,
+            layer: usize,
+            scale: f32,
+            query: *const c_void,
+            query_stride: usize,
+            output: *mut c_void,
+            output_stride: usize,
         ) -> c_int;
     }
 }

@@ -1,0 +1,411 @@
+"""CPU checks of the paged KV cache's bookkeeping and of the work lists of its
+attention calls (diskmule_amd/csrc/dm_pages.h): the header is compiled with
+the host compiler and driven with random operations and shapes, next to a
+model that is written from what the calls promise."""
+import ctypes
+import os
+import random
+import subprocess
+
+import numpy as np
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+PAGE = 64
+
+SHIM = r"""
+#include <string.h>
+#include "dm_pages.h"
+using namespace dm;
+struct Book { PageBook book; PageWork work; AttnLists lists; Book(uint32_t p, uint32_t s, uint64_t c) : book(p, s, c) {} };
+extern "C" {
+void *book_new(uint32_t p, uint32_t s, uint64_t c) { return new Book(p, s, c); }
+void book_free(Book *b) { delete b; }
+int book_create(Book *b, size_t *s) { return (int)b->book.create(s); }
+int book_extend(Book *b, size_t n, const size_t *s, const size_t *c) { return (int)b->book.extend(n, s, c, &b->work); }
+int book_fork(Book *b, size_t n, const size_t *p, const size_t *l, size_t *c) { return (int)b->book.fork(n, p, l, c, &b->work); }
+int book_truncate(Book *b, size_t s, uint64_t l) { return (int)b->book.truncate(s, l); }
+int book_release(Book *b, size_t n, const size_t *s) { return (int)b->book.release(n, s); }
+void book_compact(Book *b) { b->book.compact(&b->work); }
+uint32_t book_used(Book *b) { return b->book.used_pages(); }
+uint32_t book_row(Book *b) { return b->book.row(); }
+uint32_t book_refs(Book *b, uint32_t p) { return b->book.refs(p); }
+uint64_t book_length(Book *b, size_t s) { return b->book.at(s).length; }
+uint64_t book_version(Book *b, size_t s) { return b->book.at(s).version; }
+int book_writable(Book *b, size_t s, uint64_t n) { return b->book.writable(s, n); }
+size_t book_table(Book *b, size_t s, uint32_t *out) {
+    const auto &t = b->book.at(s).table;
+    if (out) memcpy(out, t.data(), t.size() * 4);
+    return t.size();
+}
+size_t work_copies(Book *b, uint32_t *out) {
+    if (out) memcpy(out, b->work.copies.data(), b->work.copies.size() * 8);
+    return b->work.copies.size();
+}
+size_t work_tables(Book *b, uint32_t *out) {
+    if (out) memcpy(out, b->work.tables.data(), b->work.tables.size() * 12);
+    return b->work.tables.size();
+}
+void plan(Book *b, uint32_t group, uint32_t kv_heads, uint64_t window, const uint32_t *rows, const uint32_t *wgs,
+          const uint32_t *least, uint32_t share, size_t max_parts, size_t max_bytes, size_t n, const size_t *s,
+          const size_t *c) {
+    PlanShape p;
+    p.group = group; p.kv_heads = kv_heads; p.window = window; p.share_pages = share;
+    for (int i = 0; i < 3; i++) p.rows_of[i] = rows[i], p.workgroups[i] = wgs[i], p.least_chunk[i] = least[i];
+    p.max_parts = max_parts; p.max_bytes = max_bytes;
+    Planner(b->book, p, n, s, c).build(&b->lists);
+}
+size_t lists_bytes(Book *b) { return b->lists.bytes(); }
+size_t lists_part_rows(Book *b) { return b->lists.part_rows; }
+size_t plan_least(size_t t, size_t g, size_t s) { return plan_least_bytes(t, g, s); }
+size_t list(Book *b, int which, uint32_t *out) {
+#define GIVE(v) { if (out) memcpy(out, (v).data(), (v).size() * sizeof((v)[0])); return (v).size(); }
+    if (which < 3) GIVE(b->lists.units[which])
+    if (which == 3) GIVE(b->lists.positions)
+    if (which == 4) GIVE(b->lists.joins)
+    if (which == 5) GIVE(b->lists.parts)
+    GIVE(b->lists.writes)
+}
+}
+"""
+
+OK, NO_SEQUENCE, BAD, REPEATED, CONTEXT, NO_PAGES, LENGTH = range(7)
+
+
+@pytest.fixture(scope="module")
+def lib(tmp_path_factory):
+    d = tmp_path_factory.mktemp("pages")
+    (d / "shim.cpp").write_text(SHIM)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-g", "-Wall", "-Werror", "-D_GLIBCXX_ASSERTIONS", "-shared", "-fPIC",
+                    "-I", os.path.join(ROOT, "diskmule_amd", "csrc"), str(d / "shim.cpp"), "-o", str(d / "shim.so")],
+                   check=True)
+    lib = ctypes.CDLL(str(d / "shim.so"))
+    vp, sz, u32, u64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_uint32, ctypes.c_uint64
+    lib.book_new.restype, lib.book_new.argtypes = vp, [u32, u32, u64]
+    for name, args in {"book_free": [vp], "book_create": [vp, vp], "book_extend": [vp, sz, vp, vp],
+                       "book_fork": [vp, sz, vp, vp, vp], "book_truncate": [vp, sz, u64],
+                       "book_release": [vp, sz, vp], "book_compact": [vp], "book_used": [vp], "book_row": [vp],
+                       "book_refs": [vp, u32], "book_length": [vp, sz], "book_version": [vp, sz],
+                       "book_writable": [vp, sz, u64], "book_table": [vp, sz, vp], "work_copies": [vp, vp],
+                       "work_tables": [vp, vp], "lists_bytes": [vp], "lists_part_rows": [vp],
+                       "plan_least": [sz, sz, sz], "list": [vp, ctypes.c_int, vp],
+                       "plan": [vp, u32, u32, u64, vp, vp, vp, u32, sz, sz, sz, vp, vp]}.items():
+        getattr(lib, name).argtypes = args
+    for name in ("book_table", "work_copies", "work_tables", "lists_bytes", "lists_part_rows", "plan_least", "list"):
+        getattr(lib, name).restype = sz
+    for name in ("book_length", "book_version"):
+        getattr(lib, name).restype = u64
+    for name in ("book_used", "book_row", "book_refs"):
+        getattr(lib, name).restype = u32
+    return lib
+
+
+def sizes(v):
+    return (ctypes.c_size_t * max(1, len(v)))(*v)
+
+
+class Cache:
+    """The book with a simulated device: page contents, and the table words as
+    the kernels would leave them."""
+
+    def __init__(self, lib, pages, sequences, context):
+        self.lib, self.pages, self.sequences, self.context = lib, pages, sequences, context
+        self.b = lib.book_new(pages, sequences, context)
+        self.row = lib.book_row(self.b)
+        self.memory = np.full((pages, PAGE), -1, dtype=np.int64)
+        self.words = np.zeros(sequences * self.row, dtype=np.int64)
+        self.tokens = {}  # what each live sequence holds
+        self.next = 0
+
+    def close(self):
+        self.lib.book_free(self.b)
+
+    def _work(self, name, width):
+        n = getattr(self.lib, name)(self.b, None)
+        out = np.zeros((max(n, 1), width), dtype=np.uint32)
+        getattr(self.lib, name)(self.b, out.ctypes.data)
+        return out[:n].astype(np.int64)
+
+    def device(self):
+        copies = self._work("work_copies", 2)
+        # one launch: no page is both read and written, none written twice
+        assert not set(copies[:, 0]) & set(copies[:, 1]) and len(set(copies[:, 1])) == len(copies)
+        self.memory[copies[:, 1]] = self.memory[copies[:, 0]]
+        before = self.words.copy()
+        read, written = set(), set()
+        for at, value, count in self._work("work_tables", 3):
+            assert count > 0 and at + count <= self.words.size
+            here = set(range(at, at + count))
+            assert not here & written
+            written |= here
+            if value & 0x80000000:
+                src = value & 0x7FFFFFFF
+                read |= set(range(src, src + count))
+                self.words[at:at + count] = before[src:src + count]
+            else:
+                assert value + count <= self.pages
+                self.words[at:at + count] = np.arange(value, value + count)
+        assert not read & written  # the runs of a launch may come in any order
+
+    def table(self, s):
+        out = np.zeros(self.row + 1, dtype=np.uint32)
+        n = self.lib.book_table(self.b, s, out.ctypes.data)
+        return out[:n].astype(np.int64)
+
+    def create(self):
+        s = ctypes.c_size_t()
+        r = self.lib.book_create(self.b, ctypes.byref(s))
+        if r == OK:
+            assert s.value == min(set(range(self.sequences)) - set(self.tokens))
+            self.tokens[s.value] = []
+        else:
+            assert r == NO_SEQUENCE and len(self.tokens) == self.sequences
+        return r
+
+    def extend(self, seqs, counts):
+        r = self.lib.book_extend(self.b, len(seqs), sizes(seqs), sizes(counts))
+        if r != OK:
+            return r
+        self.device()
+        for s, c in zip(seqs, counts):
+            for _ in range(c):
+                p = len(self.tokens[s])
+                self.tokens[s].append(self.next)
+                page = self.table(s)[p // PAGE]
+                assert self.lib.book_refs(self.b, page) == 1
+                self.memory[page, p % PAGE] = self.next
+                self.next += 1
+            assert self.lib.book_writable(self.b, s, c)
+        return r
+
+    def fork(self, parents, lengths):
+        out = sizes([0] * len(parents))
+        r = self.lib.book_fork(self.b, len(parents), sizes(parents), sizes(lengths), out)
+        if r == OK:
+            self.device()
+            children = list(out[:len(parents)])
+            free = sorted(set(range(self.sequences)) - set(self.tokens))
+            assert children == free[:len(children)]
+            for c, p, n in zip(children, parents, lengths):
+                self.tokens[c] = self.tokens[p][:n]
+        return r
+
+    def compact(self):
+        self.lib.book_compact(self.b)
+        moves = self._work("work_copies", 2)
+        used = self.lib.book_used(self.b)
+        assert all(moves[:, 0] >= used) and all(moves[:, 1] < used)
+        assert list(moves[:, 0]) == sorted(moves[:, 0]) and list(moves[:, 1]) == sorted(moves[:, 1])
+        self.memory[moves[:, 1]] = self.memory[moves[:, 0]]
+        self.memory[moves[:, 0]] = -2
+        to = dict(moves.tolist())
+        self.words = np.array([to.get(w, w) for w in self.words])
+
+    def check(self):
+        held = {}
+        for s, tokens in self.tokens.items():
+            assert self.lib.book_length(self.b, s) == len(tokens)
+            t = self.table(s)
+            assert len(t) == -(-len(tokens) // PAGE)
+            assert list(self.words[s * self.row:s * self.row + len(t)]) == list(t)
+            assert self.memory[t].reshape(-1)[:len(tokens)].tolist() == tokens
+            for p in t:
+                held[p] = held.get(p, 0) + 1
+        assert self.lib.book_used(self.b) == len(held)
+        for p in range(self.pages):
+            assert self.lib.book_refs(self.b, p) == held.get(p, 0)
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_random_operations_keep_every_sequences_tokens(lib, seed):
+    rng = random.Random(seed)
+    c = Cache(lib, rng.choice([6, 24, 60]), rng.choice([3, 8]), rng.choice([100, 640]))
+    for _ in range(250):
+        live = sorted(c.tokens)
+        op = rng.choice(["create", "extend", "extend", "fork", "fork", "truncate", "release", "compact"])
+        if op == "create":
+            c.create()
+        elif op == "compact":
+            c.compact()
+            used = lib.book_used(c.b)
+            assert all(p < used for s in c.tokens for p in c.table(s))
+        elif not live:
+            continue
+        elif op == "extend":
+            seqs = rng.sample(live, rng.randint(1, len(live)))
+            counts = [rng.choice([0, 1, 1, 5, 63, 64, 65, 130]) for _ in seqs]
+            before = {s: list(c.table(s)) for s in live}
+            if c.extend(seqs, counts) != OK:
+                assert before == {s: list(c.table(s)) for s in live}  # refused: nothing changed
+        elif op == "fork":
+            n = rng.randint(1, 4)
+            parents = [rng.choice(live) for _ in range(n)]
+            versions = {p: lib.book_version(c.b, p) for p in parents}
+            if c.fork(parents, [rng.randint(0, len(c.tokens[p])) for p in parents]) == OK:
+                assert all(lib.book_version(c.b, p) != v for p, v in versions.items())
+        elif op == "truncate":
+            s, n = rng.choice(live), rng.choice([0, 1, 64, 65, 100, 700])
+            assert lib.book_truncate(c.b, s, n) == OK
+            c.tokens[s] = c.tokens[s][:n]
+        else:
+            gone = rng.sample(live, rng.randint(1, len(live)))
+            assert lib.book_release(c.b, len(gone), sizes(gone)) == OK
+            for s in gone:
+                del c.tokens[s]
+        c.check()
+    c.close()
+
+
+def test_refusals_change_nothing(lib):
+    c = Cache(lib, 4, 3, 200)
+    assert c.create() == OK and c.create() == OK
+    assert c.extend([0], [130]) == OK  # three of four pages
+    for want, call in [(NO_PAGES, lambda: c.extend([1], [65])), (CONTEXT, lambda: c.extend([0], [71])),
+                       (CONTEXT, lambda: c.extend([0], [2 ** 64 - 1])), (REPEATED, lambda: c.extend([1, 1], [1, 1])),
+                       (BAD, lambda: c.extend([2], [1])), (BAD, lambda: c.extend([7], [1])),
+                       (LENGTH, lambda: c.fork([0], [131])), (BAD, lambda: c.fork([2], [0])),
+                       (NO_SEQUENCE, lambda: c.fork([0, 0], [0, 0])),
+                       (BAD, lambda: lib.book_release(c.b, 1, sizes([2]))),
+                       (REPEATED, lambda: lib.book_release(c.b, 2, sizes([0, 0]))),
+                       (BAD, lambda: lib.book_truncate(c.b, 2, 0))]:
+        version = lib.book_version(c.b, 0)
+        assert call() == want
+        assert lib.book_version(c.b, 0) == version
+        c.check()
+    assert c.fork([0], [130]) == OK  # the last page
+    assert c.fork([0], [0]) == NO_SEQUENCE
+    assert not lib.book_writable(c.b, 0, 67)  # the second page is shared now
+    assert lib.book_writable(c.b, 0, 2)
+    c.close()
+
+
+def test_a_shared_partial_page_is_copied_before_it_grows(lib):
+    c = Cache(lib, 8, 2, 512)
+    c.create()
+    c.extend([0], [128])
+    c.fork([0], [128])  # two whole pages, shared
+    lib.book_truncate(c.b, 1, 100)
+    c.tokens[1] = c.tokens[1][:100]
+    assert c.extend([1], [1]) == OK
+    assert c.table(0)[0] == c.table(1)[0] and c.table(0)[1] != c.table(1)[1]
+    c.check()
+    c.close()
+
+
+# ---- work lists ------------------------------------------------------------------
+
+def lists(lib, b, which, width):
+    n = lib.list(b, which, None)
+    out = np.zeros((max(n, 1), width), dtype=np.uint32)
+    lib.list(b, which, out.ctypes.data)
+    return out[:n].astype(np.int64)
+
+
+def check_plan(lib, c, seqs, counts, group, kv_heads, window, rows, wgs, least, share, max_parts, max_bytes):
+    """Every row sees every position that it should see exactly once, and every
+    part of a row is joined exactly once."""
+    arr = lambda v: (ctypes.c_uint32 * 3)(*v)  # noqa: E731
+    lib.plan(c.b, group, kv_heads, window, arr(rows), arr(wgs), arr(least), share, max_parts, max_bytes, len(seqs),
+             sizes(seqs), sizes(counts))
+    positions = lists(lib, c.b, 3, 1)[:, 0]
+    joins, parts, writes = lists(lib, c.b, 4, 4), lists(lib, c.b, 5, 1)[:, 0], lists(lib, c.b, 6, 4)
+    part_rows = lib.lists_part_rows(c.b)
+    want = [p for s, n in zip(seqs, counts) for p in range(len(c.tokens[s]) - n, len(c.tokens[s]))]
+    owner = [s for s, n in zip(seqs, counts) for _ in range(n)]
+    assert positions.tolist() == want
+    longest = max(len(c.tokens[s]) for s in seqs)
+    seen = [np.zeros((len(want) * group, longest), dtype=np.int8) for _ in range(1)][0]
+    part_of, final = {}, np.zeros(len(want) * group, dtype=int)
+    for cls in range(3):
+        for row0, n, seq, kv0, kv1, full0, full1, part in lists(lib, c.b, cls, 8):
+            assert 0 < n <= rows[cls] and kv0 % PAGE == 0 and kv0 < kv1
+            for r in range(row0, row0 + n):
+                p, s = positions[r // group], owner[r // group]
+                lo, hi = max(0, p + 1 - window) if window else 0, p + 1
+                assert full0 >= lo and full1 <= hi  # all rows see [full0, full1)
+                a, b = max(lo, kv0), min(hi, kv1)
+                if a < b:
+                    assert list(c.table(seq)[a // PAGE:(b - 1) // PAGE + 1]) == \
+                        list(c.table(s)[a // PAGE:(b - 1) // PAGE + 1])
+                    seen[r, a:b] += 1
+                if part == 0xFFFFFFFF:
+                    final[r] += 1
+                else:
+                    slot = part + r - row0
+                    assert slot not in part_of and slot < part_rows
+                    part_of[slot] = r
+            assert kv1 <= -(-longest // PAGE) * PAGE
+    for r in range(len(want) * group):
+        p = positions[r // group]
+        lo = max(0, p + 1 - window) if window else 0
+        assert (seen[r, lo:p + 1] == 1).all() and seen[r].sum() == p + 1 - lo
+    joined = set()
+    for row0, n, first, count in joins:
+        assert n > 0 and count > 0
+        for r in range(row0, row0 + n):
+            final[r] += 1
+            for i in range(count):
+                slot = (parts[first + i] + r) % 2 ** 32
+                assert part_of[slot] == r and slot not in joined
+                joined.add(slot)
+    assert joined == set(part_of) and (final == 1).all()
+    token = 0
+    for (token0, n, word, slot0) in writes:
+        assert token0 == token and 0 < n and slot0 + n <= PAGE
+        s = owner[token]
+        assert word == s * c.row + positions[token] // PAGE and slot0 == positions[token] % PAGE
+        assert all(o == s for o in owner[token:token + n])
+        token += n
+    assert token == len(want)
+    assert lib.lists_bytes(c.b) <= max(max_bytes, lib.plan_least(len(want), group, len(seqs)))
+    assert part_rows <= max_parts
+    return part_rows
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_work_lists_cover_what_each_row_sees_once(lib, seed):
+    rng = random.Random(1000 + seed)
+    c = Cache(lib, 400, 16, 1500)
+    c.create()
+    c.extend([0], [rng.choice([1, 64, 200, 500])])
+    for _ in range(rng.randint(0, 3)):  # a tree of prefixes
+        live = sorted(c.tokens)
+        n = rng.randint(1, 4)
+        parents = [rng.choice(live) for _ in range(n)]
+        if c.fork(parents, [rng.choice([len(c.tokens[p]), len(c.tokens[p]) // 2]) for p in parents]) != OK:
+            continue
+        c.extend(sorted(c.tokens), [rng.choice([0, 1, 70, 130]) for _ in c.tokens])
+    seqs = sorted(c.tokens)
+    if rng.random() < 0.3:
+        rng.shuffle(seqs)
+    most = rng.choice([1, 1, 6, 300])
+    counts = [min(len(c.tokens[s]), rng.randint(0 if len(seqs) > 1 else 1, most)) for s in seqs]
+    if not sum(counts):
+        counts[-1] = min(1, len(c.tokens[seqs[-1]]))
+    if not sum(counts):
+        c.extend([seqs[0]], [1])
+        counts[0] = 1
+    group = rng.choice([1, 2, 3, 4, 8, 17])
+    rows = rng.choice([[16, 64, 0], [16, 32, 0], [16, 0, 0], [16, 64, 128], [16, 64, 256]])
+    wgs = [rng.choice([1, 8, 64, 512])] * 3
+    least = [rng.choice([64, 128, 256])] * 3
+    window = rng.choice([0, 0, 1, 63, 64, 100, 5000])
+    room = rng.choice([10 ** 9, 10 ** 9, 500, 0])
+    check_plan(lib, c, seqs, counts, group, rng.choice([1, 2, 8]), window, rows, wgs, least, rng.choice([1, 2, 4]),
+               room, rng.choice([10 ** 9, 10 ** 9, 20000]))
+    c.close()
+
+
+def test_a_shared_prefix_is_one_unit_for_all(lib):
+    c = Cache(lib, 200, 9, 4096)
+    c.create()
+    c.extend([0], [1000])
+    c.fork([0] * 8, [1000] * 8)
+    c.extend(list(range(1, 9)), [1] * 8)
+    check_plan(lib, c, list(range(1, 9)), [1] * 8, 4, 2, 0, [16, 64, 0], [1] * 3, [4096] * 3, 2, 10 ** 9, 10 ** 9)
+    units = np.concatenate([lists(lib, c.b, k, 8) for k in range(3)])
+    shared = [u for u in units if u[1] == 32]
+    assert len(shared) == 1 and shared[0][3] == 0 and shared[0][4] == 15 * PAGE
+    # each sequence's own: the partly filled page and its token
+    assert sorted(tuple(u[3:5]) for u in units if u[1] != 32) == [(15 * PAGE, 1001)] * 8
+    c.close()
