@@ -25,11 +25,18 @@ constexpr uint32_t kSplitWaves = 4;
 // A page type's products: A is 16 keys (or 16 dims of values) by 32, B is 32
 // by 16 rows; lane l holds A's row and B's column l % 16, elements 8 (l / 16)
 // .. + 7, and of the result column l % 16, rows 4 (l / 16) .. + 3.
+// The wide ones: 32 by 16 times 16 by 32; lane l holds A's row and B's column
+// l % 32, elements 8 (l / 32) .. + 7, and of the result column l % 32, rows
+// 8 (i / 4) + 4 (l / 32) + i % 4.
 template <bool BF>
 struct Page;
 template <>
 struct Page<true> {
     typedef __bf16 T;
+    static __device__ __forceinline__ floatx16 mfma_wide(u32x4 a, u32x4 b, floatx16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    }
     static __device__ __forceinline__ floatx4 mfma(u32x4 a, u32x4 b, floatx4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
                                                        0, 0, 0);
@@ -38,6 +45,10 @@ struct Page<true> {
 template <>
 struct Page<false> {
     typedef _Float16 T;
+    static __device__ __forceinline__ floatx16 mfma_wide(u32x4 a, u32x4 b, floatx16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0,
+                                                      0, 0);
+    }
     static __device__ __forceinline__ floatx4 mfma(u32x4 a, u32x4 b, floatx4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0,
                                                       0, 0);
@@ -55,9 +66,11 @@ __device__ __forceinline__ float load_one(const void *p, uint32_t type, uint64_t
     return type == kBF16 ? __uint_as_float((uint32_t)b << 16) : (float)__builtin_bit_cast(_Float16, b);
 }
 
-// Eight consecutive values, of any alignment their type allows.
-__device__ __forceinline__ void load_eight(const void *p, uint32_t type, uint64_t i, float *v) {
-    if (type == kF32) {
+// Eight consecutive query values, 32-bit or of the page type, of any alignment
+// their type allows.
+template <bool BF>
+__device__ __forceinline__ void load_eight(const void *p, bool f32, uint64_t i, float *v) {
+    if (f32) {
         const f32x4a4 a = *(const f32x4a4 *)((const float *)p + i), b = *(const f32x4a4 *)((const float *)p + i + 4);
 #pragma unroll
         for (int k = 0; k < 4; k++) v[k] = a[k], v[k + 4] = b[k];
@@ -66,13 +79,8 @@ __device__ __forceinline__ void load_eight(const void *p, uint32_t type, uint64_
     const u32x4a2 w = *(const u32x4a2 *)((const uint16_t *)p + i);
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-        if (type == kBF16) {
-            v[2 * k] = __uint_as_float(w[k] << 16);
-            v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-        } else {
-            v[2 * k] = (float)__builtin_bit_cast(_Float16, (uint16_t)w[k]);
-            v[2 * k + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[k] >> 16));
-        }
+        v[2 * k] = BF ? __uint_as_float(w[k] << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)w[k]);
+        v[2 * k + 1] = BF ? __uint_as_float(w[k] & 0xffff0000u) : (float)__builtin_bit_cast(_Float16, (uint16_t)(w[k] >> 16));
     }
 }
 
@@ -108,6 +116,25 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 // of operands at a time, not all that could be asked for at once.
 __device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
 
+// 16 bytes of each lane's address straight to LDS, lane l's to dst + 16 l; the
+// wave counts it like a load.
+__device__ __forceinline__ void to_lds(const void *src, void *dst) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
+                                     (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+}
+// What this wave has asked for with to_lds has arrived, and then what every
+// wave has; and every wave is done with what it read from LDS before.
+__device__ __forceinline__ void page_arrived() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// A word that is the same for the whole wave, by the scalar path.
+__device__ __forceinline__ uint32_t word_at(const uint32_t *p, uint32_t i) {
+    return ((const __attribute__((address_space(4))) uint32_t *)p)[i];
+}
+
 // The positions a query at `position` sees: [lo, hi).
 __device__ __forceinline__ void seen(const AttnCall &c, uint32_t position, uint32_t &lo, uint32_t &hi) {
     hi = position + 1;
@@ -133,7 +160,9 @@ __device__ __forceinline__ const PlanHeader &head_of(const AttnCall &c) { return
 template <bool BF>
 __device__ void careful_rows(const AttnCall &c, const AttnUnit &u, uint32_t h, uint32_t waves, const uint32_t *again) {
     typedef typename Page<BF>::T T;
-    const uint32_t lane = threadIdx.x & 63u, hd = c.kv.head_dim;
+    uint32_t lane = threadIdx.x & 63u;
+    asm volatile("" : "+v"(lane));  // nothing of this is worked out ahead, in registers the products need
+    const uint32_t hd = c.kv.head_dim;
     const uint32_t *positions = (const uint32_t *)(c.plan + head_of(c).position_at);
     for (uint32_t r = threadIdx.x >> 6; r < u.rows; r += waves) {
         if (!again[r]) continue;
@@ -218,7 +247,8 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
     __shared__ float row_scale[kRows];
     __shared__ float2 wave_ml[kSplitWaves][kRows];
     __shared__ uint32_t again[kRows], any_again;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, n16 = lane & 15u, g = lane >> 4;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, n16 = lane & 15u, g = lane >> 4;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const uint32_t hd = c.kv.head_dim, kvh = c.kv.kv_heads;
     const PlanHeader &head = head_of(c);
     const AttnUnit *units = (const AttnUnit *)(c.plan + head.unit_at[cls]);
@@ -246,7 +276,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
                 if (there)
                     for (uint32_t ch = sub; ch < hd / 8; ch += kPer) {
                         float v[8];
-                        load_eight(c.q, c.q_type, q0 + ch * 8, v);
+                        load_eight<BF>(c.q, true, q0 + ch * 8, v);
 #pragma unroll
                         for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(v[k]));
                     }
@@ -255,12 +285,18 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
                 if (top > 0.0f && finite(top)) e = (int)(__float_as_uint(top) >> 23) - 127 - 14;
             }
             if (sub == 0) row_scale[r] = ldexpf(c.scale, e);
-#pragma unroll 1
-            for (uint32_t ch = sub; ch < D / 8; ch += kPer) {
-                float v[8];
+            constexpr int kChunks = (D / 8 + kPer - 1) / kPer;  // of a thread
+            float all[kChunks][8];
 #pragma unroll
-                for (int k = 0; k < 8; k++) v[k] = 0.0f;
-                if (there && ch < hd / 8) load_eight(c.q, c.q_type, q0 + ch * 8, v);
+            for (int i = 0; i < kChunks; i++)  // every lane loads, so that the loads go out together
+                load_eight<BF>(c.q, c.q_type == kF32, q0 + min(sub + i * kPer, hd / 8 - 1) * 8, all[i]);
+#pragma unroll
+            for (int i = 0; i < kChunks; i++) {
+                const uint32_t ch = sub + i * kPer;
+                if (D / 8 % kPer && ch >= D / 8) break;
+                float *v = all[i];
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] = there && ch < hd / 8 ? v[k] : 0.0f;
                 if (!BF && e != 0) {
 #pragma unroll
                     for (int k = 0; k < 8; k++) v[k] = ldexpf(v[k], -e);
@@ -303,10 +339,11 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
 
         const uint32_t *table = c.kv.table + (uint64_t)u.seq * c.kv.row;
         const uint32_t blocks = (u.kv1 + 31) / 32;
+        uint32_t page = word_at(table, min(u.kv0 / 32 + wave, blocks - 1) >> 1);  // a block ahead
 #pragma unroll 1
         for (uint32_t b = u.kv0 / 32 + wave; b < blocks; b += kSplitWaves) {
-            const uint32_t page = (uint32_t)__builtin_amdgcn_readfirstlane((int)table[b >> 1]);
             const T *kp = (const T *)c.kv.base + ((uint64_t)page * kvh + h) * 2 * hd * kPageTokens;
+            page = word_at(table, min(b + kSplitWaves, blocks - 1) >> 1);
             const T *vp = kp + hd * kPageTokens + ((b & 1) * 4 + g) * hd * 8;
             // Scores of 32 keys: row 4 g + i of half a is key
             // 16 (g / 2) + 4 (g % 2) + i + 8 a, so that a lane's eight are the
@@ -456,6 +493,208 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
     }
 }
 
+// Units of many rows, 16-bit results: each wave has 32 rows, all waves go
+// through the same positions a page at a time.  The page's keys and values
+// come to LDS by the memory's own path, a page ahead; a lane's scores are
+// those of one row, and in the order in which the values' operand has its
+// tokens, so that probabilities go from the scores' registers into the second
+// product as they are, and m and the sum are one number a lane.
+//
+// QT: values of the page type that a query is split into (two for a 32-bit
+// query, whose rounding would be the largest error of the result).
+template <bool BF, int D, int QT, int NW>
+__global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(AttnCall c, uint32_t cls) {
+    typedef typename Page<BF>::T T;
+    constexpr int kRows = 32 * NW, KS = D / 16, DB = D / 32;
+    constexpr int kHalf = D * kPageTokens * 2;  // bytes of a page's keys in LDS, and of its values
+    constexpr float kLift = BF ? 0.0f : 10.0f, kSlack = 5.0f;
+    extern __shared__ __attribute__((aligned(16))) uint8_t stage[];  // [2][keys, values]
+    __shared__ uint32_t again[kRows], any_again;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, n32 = lane & 31u, half = lane >> 5;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+    const uint32_t hd = c.kv.head_dim, kvh = c.kv.kv_heads;
+    const PlanHeader &head = head_of(c);
+    const AttnUnit *units = (const AttnUnit *)(c.plan + head.unit_at[cls]);
+    const uint32_t *positions = (const uint32_t *)(c.plan + head.position_at);
+    const uint32_t total = head.unit_count[cls] * kvh;
+    // key dims that the pages do not hold are zero for good: no page is copied there
+    for (uint32_t i = hd * kPageTokens * 2 + tid * 16; i < (uint32_t)kHalf; i += 64 * NW * 16)
+        *(u32x4 *)(stage + i) = *(u32x4 *)(stage + 2 * kHalf + i) = u32x4{0, 0, 0, 0};
+
+    for (uint32_t job = blockIdx.x; job < total; job += gridDim.x) {
+        const uint32_t h = job % kvh;
+        const AttnUnit u = units[job / kvh];
+        if (tid < kRows) again[tid] = 0;
+        if (tid == 0) any_again = 0;
+        const uint32_t *table = c.kv.table + (uint64_t)u.seq * c.kv.row;
+        const auto fetch = [&](uint32_t page, uint32_t buffer) {
+            const uint8_t *src = (const uint8_t *)c.kv.base + ((uint64_t)page * kvh + h) * (hd * kPageTokens * 4) + lane * 16;
+            uint8_t *dst = stage + buffer * 2 * kHalf;
+            const uint32_t pieces = hd / 8;  // KiB of keys, and of values
+#pragma unroll
+            for (uint32_t k = 0; k < D / 4 / NW; k++) {
+                const uint32_t i = k * NW + wave;
+                if (i < 2 * pieces) to_lds(src + i * 1024, dst + (i < pieces ? i * 1024 : kHalf + (i - pieces) * 1024));
+            }
+        };
+        fetch(word_at(table, u.kv0 / kPageTokens), 0);
+        const uint32_t last = (u.kv1 - 1) / kPageTokens;
+        uint32_t next_page = word_at(table, min(u.kv0 / kPageTokens + 1, last));
+        // ---- queries: this lane's row, dims 16 s + 8 half .. + 7 ----
+        const uint32_t r = wave * 32 + n32;
+        const bool there = r < u.rows;
+        const RowAt at = row_at(c, u.row0 + (there ? r : 0), h);
+        uint32_t lo = 0, hi = 0xffffffffu;
+        if (there) seen(c, positions[at.token], lo, hi);
+        u32x4 q[QT][KS];
+        float scale = c.scale;
+        {
+            const uint64_t q0 = at.token * c.q_stride + (uint64_t)at.head * hd;
+            int e = 0;
+            if (!BF && QT == 2) {  // as in attn_split_kernel
+                float top = 0.0f;
+                for (uint32_t ch = half; ch < hd / 8; ch += 2) {
+                    float v[8];
+                    load_eight<BF>(c.q, true, q0 + ch * 8, v);
+#pragma unroll
+                    for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(v[k]));
+                }
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                if (top > 0.0f && finite(top)) e = (int)(__float_as_uint(top) >> 23) - 127 - 14;
+            }
+            scale = ldexpf(scale, e);
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                if (s % 4 == 0) in_order();
+                const uint32_t ch = 2 * s + half;
+                float v[8];
+                // every lane loads, so that the loads go out together
+                load_eight<BF>(c.q, QT == 2, q0 + min(ch, hd / 8 - 1) * 8, v);
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] = there && ch * 8 < hd ? v[k] : 0.0f;
+                if (!BF && QT == 2) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) v[k] = ldexpf(v[k], -e);
+                }
+#pragma unroll
+                for (int term = 0; term < QT; term++) {
+                    T t[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        t[k] = (T)v[k];
+                        v[k] = v[k] - (float)t[k];
+                    }
+                    q[term][s] = u32x4{pack2(t[0], t[1]), pack2(t[2], t[3]), pack2(t[4], t[5]), pack2(t[6], t[7])};
+                }
+            }
+        }
+        floatx16 acc[DB];
+#pragma unroll
+        for (int db = 0; db < DB; db++) acc[db] = floatx16{};
+        float m = -INFINITY, l = 0.0f;  // l: of this lane's tokens
+
+        uint32_t buffer = 0;
+#pragma unroll 1
+        for (uint32_t t0 = u.kv0; t0 < u.kv1; t0 += kPageTokens, buffer ^= 1) {
+            page_arrived();
+            if (t0 + kPageTokens < u.kv1) {
+                fetch(next_page, buffer ^ 1);
+                next_page = word_at(table, min(t0 / kPageTokens + 2, last));
+            }
+            const uint8_t *keys = stage + buffer * 2 * kHalf + (half * 64 + n32) * 16;
+            const uint8_t *values = stage + buffer * 2 * kHalf + kHalf + (half * hd + n32) * 16;
+            floatx16 s[2] = {floatx16{}, floatx16{}};
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                if (D > 128 && ks % 4 == 0) in_order();
+#pragma unroll
+                for (int tb = 0; tb < 2; tb++) {
+                    const u32x4 k = *(const u32x4 *)(keys + ks * 2048 + tb * 512);
+#pragma unroll
+                    for (int term = 0; term < QT; term++) s[tb] = Page<BF>::mfma_wide(k, q[term][ks], s[tb]);
+                }
+            }
+            if (!(t0 >= u.full0 && t0 + kPageTokens <= u.full1)) {
+#pragma unroll
+                for (int tb = 0; tb < 2; tb++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const uint32_t t = t0 + tb * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
+                        s[tb][i] = t >= lo && t < hi ? s[tb][i] : -INFINITY;
+                    }
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int i = 1; i < 32; i++) top = fmaxf(top, s[i >> 4][i & 15]);
+            top *= scale;
+            if (__any(top > m + kSlack)) {
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float next = fmaxf(m, top);
+                const float keep = m == next ? 1.0f : exp2_hw(m - next);
+                m = next;
+                l *= keep;
+#pragma unroll
+                for (int db = 0; db < DB; db++) acc[db] = acc[db] * keep;
+            }
+            const float from = kLift - (m == -INFINITY ? 0.0f : m);
+            u32x4 p[4];
+#pragma unroll
+            for (int st = 0; st < 4; st++) {
+                T t[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float x = exp2_hw(__builtin_fmaf(s[st >> 1][(st & 1) * 8 + k], scale, from));
+                    l += x;
+                    t[k] = (T)x;
+                }
+                p[st] = u32x4{pack2(t[0], t[1]), pack2(t[2], t[3]), pack2(t[4], t[5]), pack2(t[6], t[7])};
+            }
+#pragma unroll
+            for (int st = 0; st < 4; st++) {
+                if (D > 128) in_order();
+#pragma unroll
+                for (int db = 0; db < DB; db++)
+                    acc[db] = Page<BF>::mfma_wide(*(const u32x4 *)(values + (st * 2 * hd + db * 32) * 16), p[st], acc[db]);
+            }
+        }
+
+        l += __shfl_xor(l, 32, 64);
+        uint32_t row = u.row0 + (there ? r : 0);
+        asm volatile("" : "+v"(row));  // found again here rather than kept in registers all along
+        const RowAt to = row_at(c, row, h);
+        bool odd = false;
+#pragma unroll
+        for (int db = 0; db < DB; db++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) odd |= db * 32 + 8 * (i >> 2) < (int)hd && !finite(acc[db][i]);
+        if (there) {
+            if (odd && finite(l)) again[r] = any_again = 1;
+            const bool direct = u.part == kNoPart;
+            const uint64_t slot = (uint64_t)(u.part + r) * kvh + h;
+            if (half == 0) {
+                if (!direct) c.part_ml[slot] = float2{m - kLift, l};
+                if (direct && !(l > 0.0f)) *c.bad.word = c.bad.mark;
+            }
+            const float over = 1.0f / l;
+#pragma unroll
+            for (int db = 0; db < DB; db++)
+#pragma unroll
+                for (int a = 0; a < 4; a++) {
+                    const uint32_t d = db * 32 + a * 8 + half * 4;
+                    if (d >= hd) continue;
+                    const floatx4 o = {acc[db][a * 4], acc[db][a * 4 + 1], acc[db][a * 4 + 2], acc[db][a * 4 + 3]};
+                    if (direct)
+                        store_four(c.out, c.out_type, to.token * c.out_stride + (uint64_t)to.head * hd + d, o * over);
+                    else
+                        *(f32x4a4 *)(c.part_o + slot * hd + d) = o;
+                }
+        }
+        __syncthreads();
+        if (any_again) careful_rows<BF>(c, u, h, NW, again);
+        __syncthreads();
+    }
+}
+
 // Rows whose positions were shared out: one wave a row and KV head.
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnCall c) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
@@ -500,8 +739,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnCall c) {
 
 static constexpr int some_blocks(int d) { return d <= 128 ? 4 : 2; }
 
+static constexpr int tile_waves(int d) { return 4; }
+
 uint32_t attn_pages_rows(uint32_t cls, uint32_t head_dim, bool exact) {
     if (cls == 0) return 16;
+    if (cls == 2) return exact || head_dim > 256 ? 0 : 32 * tile_waves(head_dim <= 128 ? 128 : 256);
     if (cls == 1 && head_dim <= 256) return 16 * some_blocks(head_dim <= 128 ? 128 : 256);
     return 0;
 }
@@ -515,6 +757,29 @@ static hipError_t launch_split(hipStream_t s, uint32_t cls, uint32_t grid, const
     return hipGetLastError();
 }
 
+template <bool BF, int D, int QT>
+static hipError_t launch_tile(hipStream_t s, uint32_t cls, uint32_t grid, const AttnCall &call) {
+    constexpr uint32_t kLds = 2 * 2 * D * kPageTokens * 2;
+    static LdsLimit limit;
+    const hipError_t e = limit.ensure((const void *)attn_tile_kernel<BF, D, QT, tile_waves(D)>, kLds);
+    if (e != hipSuccess) return e;
+    attn_tile_kernel<BF, D, QT, tile_waves(D)><<<grid, 64 * tile_waves(D), kLds, s>>>(call, cls);
+    return hipGetLastError();
+}
+
+template <bool BF>
+static hipError_t launch_tile_dim(hipStream_t s, uint32_t cls, uint32_t grid, const AttnCall &call) {
+    const uint32_t hd = call.kv.head_dim;
+    if (call.q_type == kF32) {
+        if (hd <= 64) return launch_tile<BF, 64, 2>(s, cls, grid, call);
+        if (hd <= 128) return launch_tile<BF, 128, 2>(s, cls, grid, call);
+        return launch_tile<BF, 256, 2>(s, cls, grid, call);
+    }
+    if (hd <= 64) return launch_tile<BF, 64, 1>(s, cls, grid, call);
+    if (hd <= 128) return launch_tile<BF, 128, 1>(s, cls, grid, call);
+    return launch_tile<BF, 256, 1>(s, cls, grid, call);
+}
+
 template <bool BF, bool EXACT>
 static hipError_t launch_dim(hipStream_t s, uint32_t cls, uint32_t grid, const AttnCall &call) {
     const uint32_t hd = call.kv.head_dim;
@@ -525,6 +790,7 @@ static hipError_t launch_dim(hipStream_t s, uint32_t cls, uint32_t grid, const A
 }
 
 hipError_t launch_attn_pages(hipStream_t s, uint32_t cls, bool bf16, bool exact, uint32_t grid, const AttnCall &call) {
+    if (cls == 2) return bf16 ? launch_tile_dim<true>(s, cls, grid, call) : launch_tile_dim<false>(s, cls, grid, call);
     if (bf16) return exact ? launch_dim<true, true>(s, cls, grid, call) : launch_dim<true, false>(s, cls, grid, call);
     return exact ? launch_dim<false, true>(s, cls, grid, call) : launch_dim<false, false>(s, cls, grid, call);
 }
