@@ -21,6 +21,9 @@ typedef uint32_t u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr uint32_t kSplitWaves = 4;
+#ifndef DM_AHEAD
+#define DM_AHEAD 0
+#endif
 
 // A page type's products: A is 16 keys (or 16 dims of values) by 32, B is 32
 // by 16 rows; lane l holds A's row and B's column l % 16, elements 8 (l / 16)
@@ -55,9 +58,26 @@ struct Page<false> {
     }
 };
 
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+// Two values in a dword, rounded to nearest even by one instruction.
 template <typename T>
-__device__ __forceinline__ uint32_t pack2(T lo, T hi) {
-    return (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2{lo, hi}), t2));
+}
+template <typename T>
+__device__ __forceinline__ u32x4 pack8(const float *v) {
+    return u32x4{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7])};
+}
+// The same, v left with what the rounding took away.
+template <typename T>
+__device__ __forceinline__ u32x4 split8(float *v) {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    const u32x4 w = pack8<T>(v);
+    const t8 t = __builtin_bit_cast(t8, w);
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = v[k] - (float)t[k];
+    return w;
 }
 
 __device__ __forceinline__ float load_one(const void *p, uint32_t type, uint64_t i) {
@@ -101,10 +121,19 @@ __device__ __forceinline__ void store_four(void *p, uint32_t type, uint64_t i, f
     }
     u32x2a2 w;
     if (type == kBF16)
-        w = u32x2a2{pack2((__bf16)v[0], (__bf16)v[1]), pack2((__bf16)v[2], (__bf16)v[3])};
+        w = u32x2a2{pack2<__bf16>(v[0], v[1]), pack2<__bf16>(v[2], v[3])};
     else
-        w = u32x2a2{pack2((_Float16)v[0], (_Float16)v[1]), pack2((_Float16)v[2], (_Float16)v[3])};
+        w = u32x2a2{pack2<_Float16>(v[0], v[1]), pack2<_Float16>(v[2], v[3])};
     *(u32x2a2 *)((uint16_t *)p + i) = w;
+}
+
+__device__ __forceinline__ void store_two(void *p, uint32_t type, uint64_t i, float a, float b) {
+    typedef uint32_t u32a2 __attribute__((aligned(2)));
+    typedef float f32x2a4 __attribute__((ext_vector_type(2), aligned(4)));
+    if (type == kF32)
+        *(f32x2a4 *)((float *)p + i) = f32x2a4{a, b};
+    else
+        *(u32a2 *)((uint16_t *)p + i) = type == kBF16 ? pack2<__bf16>(a, b) : pack2<_Float16>(a, b);
 }
 
 __device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
@@ -116,11 +145,11 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 // of operands at a time, not all that could be asked for at once.
 __device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
 
-// 16 bytes of each lane's address straight to LDS, lane l's to dst + 16 l; the
-// wave counts it like a load.
-__device__ __forceinline__ void to_lds(const void *src, void *dst) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
-                                     (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+// 16 bytes a lane from `offset` of a buffer straight to LDS, lane l's to dst +
+// 16 l; the wave counts it like a load.
+__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t src, uint32_t offset, void *dst, uint32_t lane) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void *)dst, 16, (int)(lane * 16),
+                                             (int)offset, 0, 0);
 }
 // What this wave has asked for with to_lds has arrived, and then what every
 // wave has; and every wave is done with what it read from LDS before.
@@ -303,16 +332,8 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
                 }
                 const uint32_t slot = (((r >> 4) * KS + (ch >> 2)) * 64 + (ch & 3) * 16 + (r & 15)) * 16;
 #pragma unroll
-                for (int term = 0; term < QT; term++) {
-                    T t[8];
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        t[k] = (T)v[k];
-                        v[k] = v[k] - (float)t[k];
-                    }
-                    *(u32x4 *)(shared + term * (NB * KS * 1024) + slot) =
-                        u32x4{pack2(t[0], t[1]), pack2(t[2], t[3]), pack2(t[4], t[5]), pack2(t[6], t[7])};
-                }
+                for (int term = 0; term < QT; term++)
+                    *(u32x4 *)(shared + term * (NB * KS * 1024) + slot) = split8<T>(v);
             }
         }
         __syncthreads();
@@ -403,21 +424,13 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
                     for (int db = 0; db < DB; db++) acc[db][nb] = acc[db][nb] * keep;
                 }
                 const float from = (m[nb] == -INFINITY ? 0.0f : m[nb]) - kLift;
-                T t[8];
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
                     x[k] = exp2_hw(x[k] - from);
                     l[nb] += x[k];
                 }
 #pragma unroll
-                for (int term = 0; term < PT; term++) {
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        t[k] = (T)x[k];
-                        x[k] = x[k] - (float)t[k];
-                    }
-                    p[term][nb] = u32x4{pack2(t[0], t[1]), pack2(t[2], t[3]), pack2(t[4], t[5]), pack2(t[6], t[7])};
-                }
+                for (int term = 0; term < PT; term++) p[term][nb] = split8<T>(x);
             }
 #pragma unroll
             for (int db = 0; db < DB; db++) {
@@ -508,7 +521,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
     constexpr int kRows = 32 * NW, KS = D / 16, DB = D / 32;
     constexpr int kHalf = D * kPageTokens * 2;  // bytes of a page's keys in LDS, and of its values
     constexpr float kLift = BF ? 0.0f : 10.0f, kSlack = 5.0f;
-    extern __shared__ __attribute__((aligned(16))) uint8_t stage[];  // [2][keys, values]
+    constexpr int kSteps = 2 * KS + 4 * DB;  // products of a page, by their first operand from LDS
+    constexpr bool kAhead = QT == 1 && DM_AHEAD;
+    extern __shared__ __attribute__((aligned(16))) uint8_t stage[];  // keys, keys, values, values
     __shared__ uint32_t again[kRows], any_again;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, n32 = lane & 31u, half = lane >> 5;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
@@ -519,7 +534,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
     const uint32_t total = head.unit_count[cls] * kvh;
     // key dims that the pages do not hold are zero for good: no page is copied there
     for (uint32_t i = hd * kPageTokens * 2 + tid * 16; i < (uint32_t)kHalf; i += 64 * NW * 16)
-        *(u32x4 *)(stage + i) = *(u32x4 *)(stage + 2 * kHalf + i) = u32x4{0, 0, 0, 0};
+        *(u32x4 *)(stage + i) = *(u32x4 *)(stage + kHalf + i) = u32x4{0, 0, 0, 0};
 
     for (uint32_t job = blockIdx.x; job < total; job += gridDim.x) {
         const uint32_t h = job % kvh;
@@ -527,19 +542,25 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
         if (tid < kRows) again[tid] = 0;
         if (tid == 0) any_again = 0;
         const uint32_t *table = c.kv.table + (uint64_t)u.seq * c.kv.row;
-        const auto fetch = [&](uint32_t page, uint32_t buffer) {
-            const uint8_t *src = (const uint8_t *)c.kv.base + ((uint64_t)page * kvh + h) * (hd * kPageTokens * 4) + lane * 16;
-            uint8_t *dst = stage + buffer * 2 * kHalf;
-            const uint32_t pieces = hd / 8;  // KiB of keys, and of values
+        // a page's keys (at 0) or values (at kHalf) into buffer 0 or 1 of them
+        const auto fetch = [&](uint32_t page, uint32_t values, uint32_t buffer) {
+            const uint32_t pieces = hd / 8;  // KiB
+            const auto src = make_rsrc((const uint8_t *)c.kv.base + ((uint64_t)page * kvh + h) * (hd * kPageTokens * 4) +
+                                           values * (hd * kPageTokens * 2),
+                                       hd * kPageTokens * 2);
+            uint8_t *dst = stage + (2 * values + buffer) * kHalf;
 #pragma unroll
-            for (uint32_t k = 0; k < D / 4 / NW; k++) {
+            for (uint32_t k = 0; k < D / 8 / NW; k++) {
                 const uint32_t i = k * NW + wave;
-                if (i < 2 * pieces) to_lds(src + i * 1024, dst + (i < pieces ? i * 1024 : kHalf + (i - pieces) * 1024));
+                if (i < pieces) to_lds(src, i * 1024, dst + i * 1024, lane);
             }
         };
-        fetch(word_at(table, u.kv0 / kPageTokens), 0);
-        const uint32_t last = (u.kv1 - 1) / kPageTokens;
-        uint32_t next_page = word_at(table, min(u.kv0 / kPageTokens + 1, last));
+        const uint32_t first = u.kv0 / kPageTokens, last = (u.kv1 - 1) / kPageTokens;
+        uint32_t page = word_at(table, first), page1 = word_at(table, min(first + 1, last));
+        uint32_t page2 = word_at(table, min(first + 2, last));
+        fetch(page, 0, 0);
+        fetch(page, 1, 0);
+        if (kAhead) fetch(page1, 0, 1);
         // ---- queries: this lane's row, dims 16 s + 8 half .. + 7 ----
         const uint32_t r = wave * 32 + n32;
         const bool there = r < u.rows;
@@ -565,7 +586,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
             scale = ldexpf(scale, e);
 #pragma unroll
             for (int s = 0; s < KS; s++) {
-                if (s % 4 == 0) in_order();
+                if (D > 128 || s % 4 == 0) in_order();
                 const uint32_t ch = 2 * s + half;
                 float v[8];
                 // every lane loads, so that the loads go out together
@@ -577,15 +598,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
                     for (int k = 0; k < 8; k++) v[k] = ldexpf(v[k], -e);
                 }
 #pragma unroll
-                for (int term = 0; term < QT; term++) {
-                    T t[8];
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        t[k] = (T)v[k];
-                        v[k] = v[k] - (float)t[k];
-                    }
-                    q[term][s] = u32x4{pack2(t[0], t[1]), pack2(t[2], t[3]), pack2(t[4], t[5]), pack2(t[6], t[7])};
-                }
+                for (int term = 0; term < QT; term++) q[term][s] = split8<T>(v);
             }
         }
         floatx16 acc[DB];
@@ -593,27 +606,59 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
         for (int db = 0; db < DB; db++) acc[db] = floatx16{};
         float m = -INFINITY, l = 0.0f;  // l: of this lane's tokens
 
-        uint32_t buffer = 0;
-#pragma unroll 1
-        for (uint32_t t0 = u.kv0; t0 < u.kv1; t0 += kPageTokens, buffer ^= 1) {
-            page_arrived();
-            if (t0 + kPageTokens < u.kv1) {
-                fetch(next_page, buffer ^ 1);
-                next_page = word_at(table, min(t0 / kPageTokens + 2, last));
-            }
-            const uint8_t *keys = stage + buffer * 2 * kHalf + (half * 64 + n32) * 16;
-            const uint8_t *values = stage + buffer * 2 * kHalf + kHalf + (half * hd + n32) * 16;
-            floatx16 s[2] = {floatx16{}, floatx16{}};
+        const auto score = [&](floatx16 *s, uint32_t buffer) {
+            const uint8_t *keys = stage + buffer * kHalf + (half * 64 + n32) * 16;
+            s[0] = s[1] = floatx16{};
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                if (D > 128 && ks % 4 == 0) in_order();
+            for (int ks = 0; ks < KS; ks++)
 #pragma unroll
                 for (int tb = 0; tb < 2; tb++) {
                     const u32x4 k = *(const u32x4 *)(keys + ks * 2048 + tb * 512);
 #pragma unroll
                     for (int term = 0; term < QT; term++) s[tb] = Page<BF>::mfma_wide(k, q[term][ks], s[tb]);
                 }
+        };
+        // first operand of product i of a turn: the keys of the page ahead, then
+        // this page's values
+        const auto operand = [&](int i, uint32_t buffer) {
+            if (i < 2 * KS)
+                return *(const u32x4 *)(stage + (kAhead ? buffer ^ 1 : buffer) * kHalf + (half * 64 + n32) * 16 + (i >> 1) * 2048 + (i & 1) * 512);
+            const int db = (i - 2 * KS) % DB, st = (i - 2 * KS) / DB;
+            return *(const u32x4 *)(stage + (2 + buffer) * kHalf + (half * hd + n32) * 16 + (st * 2 * hd + db * 32) * 16);
+        };
+        floatx16 s[2], ahead[2];
+        u32x4 ring[4];
+        if (kAhead) {
+            page_arrived();
+            score(s, 0);
+        }
+        uint32_t buffer = 0;
+#pragma unroll 1
+        for (uint32_t at_page = first; at_page <= last; at_page++, buffer ^= 1) {
+            // the next page's keys and this one's values are there; the keys
+            // this loop's last turn scored, and its values, are done with
+            page_arrived();
+            if (kAhead)
+                fetch(page2, 0, buffer);
+            else
+                fetch(page1, 0, buffer ^ 1);
+            fetch(page1, 1, buffer ^ 1);
+            page1 = page2;
+            page2 = word_at(table, min(at_page + 3, last));
+            ring[0] = operand(0, buffer);
+            ring[1] = operand(1, buffer);
+            if (!kAhead) {
+                s[0] = s[1] = floatx16{};
+#pragma unroll
+                for (int i = 0; i < 2 * KS; i++) {
+                    ring[(i + 2) % 4] = operand(i + 2, buffer);
+#pragma unroll
+                    for (int term = 0; term < QT; term++)
+                        s[i & 1] = Page<BF>::mfma_wide(ring[i % 4], q[term][i >> 1], s[i & 1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
+            const uint32_t t0 = at_page * kPageTokens;
             if (!(t0 >= u.full0 && t0 + kPageTokens <= u.full1)) {
 #pragma unroll
                 for (int tb = 0; tb < 2; tb++)
@@ -637,41 +682,73 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
                 for (int db = 0; db < DB; db++) acc[db] = acc[db] * keep;
             }
             const float from = kLift - (m == -INFINITY ? 0.0f : m);
+            // The next page's scores (the last turn's are of no use), and beside
+            // each product a share of this page's exponentials; then this page's
+            // values by its probabilities.  In this order and no other: LDS is
+            // read two operands ahead of their products.
+            float part[2] = {0.0f, 0.0f};
             u32x4 p[4];
+            const auto exponentials = [&](int e) {  // pair e of the 16
+                const float x0 = exp2_hw(__builtin_fmaf(s[e >> 3][2 * (e & 7)], scale, from));
+                const float x1 = exp2_hw(__builtin_fmaf(s[e >> 3][2 * (e & 7) + 1], scale, from));
+                part[0] += x0;
+                part[1] += x1;
+                p[e >> 2][e & 3] = pack2<T>(x0, x1);
+            };
+            if (kAhead) {
+                ahead[0] = ahead[1] = floatx16{};
 #pragma unroll
-            for (int st = 0; st < 4; st++) {
-                T t[8];
+                for (int i = 0; i < kSteps; i++) {
+                    if (i + 2 < kSteps) ring[(i + 2) % 4] = operand(i + 2, buffer);
+                    if (i < 2 * KS) {
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const float x = exp2_hw(__builtin_fmaf(s[st >> 1][(st & 1) * 8 + k], scale, from));
-                    l += x;
-                    t[k] = (T)x;
+                        for (int term = 0; term < QT; term++)
+                            ahead[i & 1] = Page<BF>::mfma_wide(ring[i % 4], q[term][i >> 1], ahead[i & 1]);
+#pragma unroll
+                        for (int e = i * 8 / KS; e < (i + 1) * 8 / KS; e++) exponentials(e);
+                    } else {
+                        const int db = (i - 2 * KS) % DB, st = (i - 2 * KS) / DB;
+                        acc[db] = Page<BF>::mfma_wide(ring[i % 4], p[st], acc[db]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                p[st] = u32x4{pack2(t[0], t[1]), pack2(t[2], t[3]), pack2(t[4], t[5]), pack2(t[6], t[7])};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) exponentials(e);
+#pragma unroll
+                for (int i = 2 * KS; i < kSteps; i++) {
+                    if (i + 2 < kSteps) ring[(i + 2) % 4] = operand(i + 2, buffer);
+                    const int j = i - 2 * KS, db = j % DB, st = j / DB;
+                    acc[db] = Page<BF>::mfma_wide(ring[i % 4], p[st], acc[db]);
+#pragma unroll
+                    for (int e = 4 + j * 4 / DB; e < 4 + (j + 1) * 4 / DB; e++)
+                        if (e < 16) exponentials(e);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
-#pragma unroll
-            for (int st = 0; st < 4; st++) {
-                if (D > 128) in_order();
-#pragma unroll
-                for (int db = 0; db < DB; db++)
-                    acc[db] = Page<BF>::mfma_wide(*(const u32x4 *)(values + (st * 2 * hd + db * 32) * 16), p[st], acc[db]);
+            l += part[0] + part[1];
+            if (kAhead) {
+                s[0] = ahead[0];
+                s[1] = ahead[1];
             }
         }
 
         l += __shfl_xor(l, 32, 64);
-        uint32_t row = u.row0 + (there ? r : 0);
-        asm volatile("" : "+v"(row));  // found again here rather than kept in registers all along
-        const RowAt to = row_at(c, row, h);
-        bool odd = false;
+        // found again here rather than kept in registers all along
+        uint32_t id = threadIdx.x;
+        asm volatile("" : "+v"(id));
+        const uint32_t r1 = (id >> 6) * 32 + (id & 31), half1 = (id >> 5) & 1;
+        if (r1 < u.rows) {
+            const RowAt to = row_at(c, u.row0 + r1, h);
+            bool odd = false;
 #pragma unroll
-        for (int db = 0; db < DB; db++)
+            for (int db = 0; db < DB; db++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) odd |= db * 32 + 8 * (i >> 2) < (int)hd && !finite(acc[db][i]);
-        if (there) {
-            if (odd && finite(l)) again[r] = any_again = 1;
+                for (int i = 0; i < 16; i++) odd |= db * 32 + 8 * (i >> 2) < (int)hd && !finite(acc[db][i]);
+            if (odd && finite(l)) again[r1] = any_again = 1;
             const bool direct = u.part == kNoPart;
-            const uint64_t slot = (uint64_t)(u.part + r) * kvh + h;
-            if (half == 0) {
+            const uint64_t slot = (uint64_t)(u.part + r1) * kvh + h;
+            if (half1 == 0) {
                 if (!direct) c.part_ml[slot] = float2{m - kLift, l};
                 if (direct && !(l > 0.0f)) *c.bad.word = c.bad.mark;
             }
@@ -680,7 +757,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
             for (int db = 0; db < DB; db++)
 #pragma unroll
                 for (int a = 0; a < 4; a++) {
-                    const uint32_t d = db * 32 + a * 8 + half * 4;
+                    const uint32_t d = db * 32 + a * 8 + half1 * 4;
                     if (d >= hd) continue;
                     const floatx4 o = {acc[db][a * 4], acc[db][a * 4 + 1], acc[db][a * 4 + 2], acc[db][a * 4 + 3]};
                     if (direct)
@@ -695,45 +772,57 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
     }
 }
 
-// Rows whose positions were shared out: one wave a row and KV head.
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnCall c) {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+// Rows whose positions were shared out: one wave a row, a lane V dims of it. A
+// lane first takes a part's m and sum, 64 parts at once, and then hands the
+// part's weight to all, so that the loads of the parts' o wait for nothing.
+template <int V>
+__global__ __launch_bounds__(64 * kJoinRows) void attn_join_kernel(AttnCall c) {
+    typedef float floatv __attribute__((ext_vector_type(V), aligned(4)));
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t hd = c.kv.head_dim, kvh = c.kv.kv_heads;
     const PlanHeader &head = head_of(c);
     const JoinItem *items = (const JoinItem *)(c.plan + head.join_at);
     const uint32_t *parts = (const uint32_t *)(c.plan + head.part_at);
     const uint32_t total = head.join_count * kvh;
+    const uint32_t d = lane * V < hd ? lane * V : 0;  // lanes past the head do the first dims' work again
     for (uint32_t job = blockIdx.x; job < total; job += gridDim.x) {
         const uint32_t h = job % kvh;
         const JoinItem it = items[job / kvh];
-        for (uint32_t r = it.row0 + wave; r < it.row0 + it.rows; r += 4) {
-            float top = -INFINITY;
-            for (uint32_t i = 0; i < it.count; i++)
-                top = fmaxf(top, c.part_ml[(uint64_t)(parts[it.first + i] + r) * kvh + h].x);
-            float sum = 0.0f;
-            float o[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) o[e] = 0.0f;
-            for (uint32_t i = 0; i < it.count; i++) {
-                const uint64_t slot = (uint64_t)(parts[it.first + i] + r) * kvh + h;
-                const float2 ml = c.part_ml[slot];
-                if (ml.y == 0.0f) continue;  // saw nothing
-                const float f = ml.x == top ? 1.0f : exp2_hw(ml.x - top);
+        if (wave >= it.rows) continue;
+        const uint32_t r = it.row0 + wave;
+        float top = -INFINITY;
+        for (uint32_t i = lane; i < it.count; i += 64)
+            top = fmaxf(top, c.part_ml[(uint64_t)(parts[it.first + i] + r) * kvh + h].x);
+        top = wave_max(top);
+        float sum = 0.0f;
+        floatv o = 0.0f;
+        for (uint32_t i0 = 0; i0 < it.count; i0 += 64) {
+            const uint32_t n = min(64u, it.count - i0);
+            const uint32_t slot = lane < n ? parts[it.first + i0 + lane] + r : 0;
+            float f = 0.0f;
+            if (lane < n) {
+                const float2 ml = c.part_ml[(uint64_t)slot * kvh + h];
+                // a part that saw nothing has no weight, whatever m is
+                f = ml.y == 0.0f ? 0.0f : ml.x == top ? 1.0f : exp2_hw(ml.x - top);
                 sum += ml.y * f;
-#pragma unroll
-                for (uint32_t e = 0; e < 8; e++) {
-                    const uint32_t d = e * 64 + lane;
-                    if (d < hd) o[e] = __builtin_fmaf(f, c.part_o[slot * hd + d], o[e]);
-                }
             }
-            const RowAt at = row_at(c, r, h);
-            if (lane == 0 && !(sum > 0.0f)) *c.bad.word = c.bad.mark;
+#pragma unroll 8
+            for (uint32_t i = 0; i < n; i++) {
+                const uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)slot, (int)i);
+                const float w = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(f), (int)i));
+                const floatv v = *(const floatv *)(c.part_o + ((uint64_t)at * kvh + h) * hd + d);
 #pragma unroll
-            for (uint32_t e = 0; e < 8; e++) {
-                const uint32_t d = e * 64 + lane;
-                if (d < hd) store_one(c.out, c.out_type, at.token * c.out_stride + (uint64_t)at.head * hd + d, o[e] / sum);
+                for (int e = 0; e < V; e++) o[e] = __builtin_fmaf(w, v[e], o[e]);
             }
         }
+        sum = wave_sum(sum);
+        if (lane == 0 && !(sum > 0.0f)) *c.bad.word = c.bad.mark;
+        const RowAt at = row_at(c, r, h);
+        const uint64_t to = at.token * c.out_stride + (uint64_t)at.head * hd + lane * V;
+        if (lane * V < hd)
+#pragma unroll
+            for (int e = 0; e < V; e += 2) store_two(c.out, c.out_type, to + e, o[e] / sum, o[e + 1] / sum);
     }
 }
 
@@ -796,10 +885,16 @@ hipError_t launch_attn_pages(hipStream_t s, uint32_t cls, bool bf16, bool exact,
 }
 
 hipError_t launch_attn_join(hipStream_t s, uint32_t grid, const AttnCall &call) {
-    attn_join_kernel<<<grid, 256, 0, s>>>(call);
+    const uint32_t hd = call.kv.head_dim;
+    if (hd <= 128)
+        attn_join_kernel<2><<<grid, 64 * kJoinRows, 0, s>>>(call);
+    else if (hd <= 256)
+        attn_join_kernel<4><<<grid, 64 * kJoinRows, 0, s>>>(call);
+    else
+        attn_join_kernel<8><<<grid, 64 * kJoinRows, 0, s>>>(call);
     return hipGetLastError();
 }
 
-const void *module_anchor_attn_pages() { return (const void *)attn_join_kernel; }
+const void *module_anchor_attn_pages() { return (const void *)attn_join_kernel<2>; }
 
 }  // namespace dm

@@ -308,8 +308,9 @@ class PageBook {
 struct AttnUnit {
     uint32_t row0, rows, seq, kv0, kv1, full0, full1, part;
 };
-// Rows whose result is joined from `count` partial results: that of row r in
-// part i stands at parts[first + i] + r (modulo 2^32).
+// Up to kJoinRows rows whose result is joined from `count` partial results: that
+// of row r in part i stands at parts[first + i] + r (modulo 2^32).
+constexpr uint32_t kJoinRows = 4;
 struct JoinItem {
     uint32_t row0, rows, first, count;
 };
@@ -570,8 +571,11 @@ class Planner {
                 for (const uint32_t p : l.parts[tile]) out_->parts.push_back(p);
             }
             item.count = (uint32_t)out_->parts.size() - item.first;
-            if (item.count) out_->joins.push_back(item);  // none: the one unit wrote its rows itself
-            r += item.rows;
+            const uint32_t to = r + item.rows;
+            if (item.count)  // none: the one unit wrote its rows itself
+                for (uint32_t a = r; a < to; a += kJoinRows)
+                    out_->joins.push_back({a, std::min(kJoinRows, to - a), item.first, item.count});
+            r = to;
             if (!plain_ && !fits()) return false;
         }
         return true;

@@ -545,7 +545,7 @@ int dmhip_new_kv_plan(dmhip_kv_pages *pool, size_t query_heads, int has_window, 
     }
     const size_t sequences = std::min<size_t>(pool->book.sequences(), max_tokens);
     s.max_parts = 2 * std::min(rows, sequences * kSharedRows) + 4 * (size_t)cus * most / pool->kv_heads + most;
-    s.max_bytes = plan_least_bytes(max_tokens, group, sequences) + (512u << 10);
+    s.max_bytes = plan_least_bytes(max_tokens, group, sequences) + rows / kJoinRows * sizeof(JoinItem) + (512u << 10);
     p->list_bytes = sizeof(PlanHeader) + s.max_bytes + 16 * 8;
     const size_t part_rows = s.max_parts * pool->kv_heads;
     const size_t sizes[3] = {p->list_bytes, part_rows * pool->head_dim * 4, part_rows * sizeof(float2)};
