@@ -21,9 +21,6 @@ typedef uint32_t u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr uint32_t kSplitWaves = 4;
-#ifndef DM_AHEAD
-#define DM_AHEAD 0
-#endif
 
 // A page type's products: A is 16 keys (or 16 dims of values) by 32, B is 32
 // by 16 rows; lane l holds A's row and B's column l % 16, elements 8 (l / 16)
@@ -159,6 +156,21 @@ __device__ __forceinline__ void page_arrived() {
     asm volatile("" ::: "memory");
 }
 
+// What every wave has written to LDS is there; loads in flight go on.
+__device__ __forceinline__ void scores_met() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// The thread's number, as if it were another for each unit: what is worked out
+// of it for one unit is not kept in registers for all of them.
+__device__ __forceinline__ uint32_t thread_here() {
+    uint32_t id = threadIdx.x;
+    asm volatile("" : "+v"(id));
+    return id;
+}
+
 // A word that is the same for the whole wave, by the scalar path.
 __device__ __forceinline__ uint32_t word_at(const uint32_t *p, uint32_t i) {
     return ((const __attribute__((address_space(4))) uint32_t *)p)[i];
@@ -180,17 +192,16 @@ __device__ __forceinline__ RowAt row_at(const AttnCall &c, uint32_t row, uint32_
 
 __device__ __forceinline__ const PlanHeader &head_of(const AttnCall &c) { return *(const PlanHeader *)c.plan; }
 
-// Rows of a unit again, with every masked product left out instead of multiplied by
-// zero, and queries and probabilities in 32 bits: for rows that met a value that
-// is not finite (marked in `again`).  Such a value in a place that a row does not see must
-// not reach its result (0 * inf), and where queries or probabilities are split
-// into terms, one that it does see gives inf - inf.  One wave a row: a lane a
-// key, then a lane a dim.
+// Rows of a unit again, with every masked product left out instead of
+// multiplied by zero, and queries and probabilities in 32 bits: for rows whose
+// sum or result is not finite (marked in `again`). A value that is not finite
+// in a place that a row does not see must not reach its result (0 * inf), and
+// one that it does see gives inf - inf where queries or probabilities are split
+// into several values. One wave a row: a lane a key, then a lane a dim.
 template <bool BF>
 __device__ void careful_rows(const AttnCall &c, const AttnUnit &u, uint32_t h, uint32_t waves, const uint32_t *again) {
     typedef typename Page<BF>::T T;
-    uint32_t lane = threadIdx.x & 63u;
-    asm volatile("" : "+v"(lane));  // nothing of this is worked out ahead, in registers the products need
+    const uint32_t lane = thread_here() & 63u;
     const uint32_t hd = c.kv.head_dim;
     const uint32_t *positions = (const uint32_t *)(c.plan + head_of(c).position_at);
     for (uint32_t r = threadIdx.x >> 6; r < u.rows; r += waves) {
@@ -258,14 +269,16 @@ __device__ void careful_rows(const AttnCall &c, const AttnUnit &u, uint32_t h, u
 // the matrix operands, and uses them for all rows, so that a unit reads what
 // its rows see once; the waves' results meet in LDS at the end.
 //
-// EXACT (32-bit results): queries and probabilities in two halves (F16) or
-// three and two (BF16), which leaves 2^-17 of a probability; otherwise each is
-// rounded to the page type once, half a step of it, as the result is.
+// EXACT (32-bit results): queries in two values of the page type (F16) or three
+// (BF16), probabilities in two, which leaves 2^-17 of a probability. Otherwise
+// queries in two, and probabilities rounded to the page type once: half a step
+// of it, as the result is; a 32-bit query's own rounding would be more, its
+// error being that of the whole score.
 template <bool BF, int D, int NB, bool EXACT>
 __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c, uint32_t cls) {
     typedef typename Page<BF>::T T;
     constexpr int kRows = 16 * NB, KS = D / 32, DB = D / 16;
-    constexpr int QT = EXACT ? (BF ? 3 : 2) : 1, PT = EXACT ? 2 : 1;
+    constexpr int QT = EXACT && BF ? 3 : 2, PT = EXACT ? 2 : 1;
     // Probabilities of F16 pages are 2^10 times larger: its smallest value 2^-24
     // would lose the many small ones of a long row.
     constexpr float kLift = BF ? 0.0f : 10.0f;
@@ -276,8 +289,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
     __shared__ float row_scale[kRows];
     __shared__ float2 wave_ml[kSplitWaves][kRows];
     __shared__ uint32_t again[kRows], any_again;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, n16 = lane & 15u, g = lane >> 4;
-    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t hd = c.kv.head_dim, kvh = c.kv.kv_heads;
     const PlanHeader &head = head_of(c);
     const AttnUnit *units = (const AttnUnit *)(c.plan + head.unit_at[cls]);
@@ -287,6 +299,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
     for (uint32_t job = blockIdx.x; job < total; job += gridDim.x) {
         const uint32_t h = job % kvh;
         const AttnUnit u = units[job / kvh];
+        const uint32_t tid = thread_here(), lane = tid & 63u, n16 = lane & 15u, g = lane >> 4;
         if (tid < kRows) again[tid] = 0;
         if (tid == 0) any_again = 0;
         // ---- queries into LDS, as the B operands of the products ----
@@ -488,10 +501,10 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
                 for (uint32_t w = 0; w < kSplitWaves; w++)
                     o += *(const floatx4 *)(reduce + (w * kRows + r) * kReducePitch + (i & 7) * 4);
                 const bool odd = !finite(o[0]) || !finite(o[1]) || !finite(o[2]) || !finite(o[3]);
-                if (EXACT ? odd || !(sum > 0.0f && finite(sum)) : odd && finite(sum)) again[r] = any_again = 1;
+                if (odd || !finite(sum)) again[r] = any_again = 1;
                 const RowAt at = row_at(c, u.row0 + r, h);
                 if (u.part == kNoPart) {
-                    if (d == 0 && !EXACT && !(sum > 0.0f)) *c.bad.word = c.bad.mark;
+                    if (d == 0 && sum == 0.0f) *c.bad.word = c.bad.mark;
                     store_four(c.out, c.out_type, at.token * c.out_stride + (uint64_t)at.head * hd + d, o / sum);
                 } else {
                     const uint64_t slot = (uint64_t)(u.part + r) * kvh + h;
@@ -522,23 +535,22 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
     constexpr int kHalf = D * kPageTokens * 2;  // bytes of a page's keys in LDS, and of its values
     constexpr float kLift = BF ? 0.0f : 10.0f, kSlack = 5.0f;
     constexpr int kSteps = 2 * KS + 4 * DB;  // products of a page, by their first operand from LDS
-    constexpr bool kAhead = QT == 1 && DM_AHEAD;
     extern __shared__ __attribute__((aligned(16))) uint8_t stage[];  // keys, keys, values, values
     __shared__ uint32_t again[kRows], any_again;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, n32 = lane & 31u, half = lane >> 5;
-    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t hd = c.kv.head_dim, kvh = c.kv.kv_heads;
     const PlanHeader &head = head_of(c);
     const AttnUnit *units = (const AttnUnit *)(c.plan + head.unit_at[cls]);
     const uint32_t *positions = (const uint32_t *)(c.plan + head.position_at);
     const uint32_t total = head.unit_count[cls] * kvh;
     // key dims that the pages do not hold are zero for good: no page is copied there
-    for (uint32_t i = hd * kPageTokens * 2 + tid * 16; i < (uint32_t)kHalf; i += 64 * NW * 16)
+    for (uint32_t i = hd * kPageTokens * 2 + threadIdx.x * 16; i < (uint32_t)kHalf; i += 64 * NW * 16)
         *(u32x4 *)(stage + i) = *(u32x4 *)(stage + kHalf + i) = u32x4{0, 0, 0, 0};
 
     for (uint32_t job = blockIdx.x; job < total; job += gridDim.x) {
         const uint32_t h = job % kvh;
         const AttnUnit u = units[job / kvh];
+        const uint32_t tid = thread_here(), lane = tid & 63u, n32 = lane & 31u, half = lane >> 5;
         if (tid < kRows) again[tid] = 0;
         if (tid == 0) any_again = 0;
         const uint32_t *table = c.kv.table + (uint64_t)u.seq * c.kv.row;
@@ -556,11 +568,10 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
             }
         };
         const uint32_t first = u.kv0 / kPageTokens, last = (u.kv1 - 1) / kPageTokens;
-        uint32_t page = word_at(table, first), page1 = word_at(table, min(first + 1, last));
-        uint32_t page2 = word_at(table, min(first + 2, last));
+        uint32_t page = word_at(table, first);
         fetch(page, 0, 0);
         fetch(page, 1, 0);
-        if (kAhead) fetch(page1, 0, 1);
+        page = word_at(table, min(first + 1, last));  // the one that is fetched next
         // ---- queries: this lane's row, dims 16 s + 8 half .. + 7 ----
         const uint32_t r = wave * 32 + n32;
         const bool there = r < u.rows;
@@ -606,57 +617,34 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
         for (int db = 0; db < DB; db++) acc[db] = floatx16{};
         float m = -INFINITY, l = 0.0f;  // l: of this lane's tokens
 
-        const auto score = [&](floatx16 *s, uint32_t buffer) {
-            const uint8_t *keys = stage + buffer * kHalf + (half * 64 + n32) * 16;
-            s[0] = s[1] = floatx16{};
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                for (int tb = 0; tb < 2; tb++) {
-                    const u32x4 k = *(const u32x4 *)(keys + ks * 2048 + tb * 512);
-#pragma unroll
-                    for (int term = 0; term < QT; term++) s[tb] = Page<BF>::mfma_wide(k, q[term][ks], s[tb]);
-                }
-        };
-        // first operand of product i of a turn: the keys of the page ahead, then
-        // this page's values
+        // first operand of product i of a page: of its keys, then of its values
         const auto operand = [&](int i, uint32_t buffer) {
             if (i < 2 * KS)
-                return *(const u32x4 *)(stage + (kAhead ? buffer ^ 1 : buffer) * kHalf + (half * 64 + n32) * 16 + (i >> 1) * 2048 + (i & 1) * 512);
+                return *(const u32x4 *)(stage + buffer * kHalf + (half * 64 + n32) * 16 + (i >> 1) * 2048 + (i & 1) * 512);
             const int db = (i - 2 * KS) % DB, st = (i - 2 * KS) / DB;
             return *(const u32x4 *)(stage + (2 + buffer) * kHalf + (half * hd + n32) * 16 + (st * 2 * hd + db * 32) * 16);
         };
-        floatx16 s[2], ahead[2];
         u32x4 ring[4];
-        if (kAhead) {
-            page_arrived();
-            score(s, 0);
-        }
         uint32_t buffer = 0;
 #pragma unroll 1
         for (uint32_t at_page = first; at_page <= last; at_page++, buffer ^= 1) {
-            // the next page's keys and this one's values are there; the keys
-            // this loop's last turn scored, and its values, are done with
             page_arrived();
-            if (kAhead)
-                fetch(page2, 0, buffer);
-            else
-                fetch(page1, 0, buffer ^ 1);
-            fetch(page1, 1, buffer ^ 1);
-            page1 = page2;
-            page2 = word_at(table, min(at_page + 3, last));
+            if (at_page < last) {
+                fetch(page, 0, buffer ^ 1);
+                fetch(page, 1, buffer ^ 1);
+            }
+            page = word_at(table, min(at_page + 2, last));
             ring[0] = operand(0, buffer);
             ring[1] = operand(1, buffer);
-            if (!kAhead) {
-                s[0] = s[1] = floatx16{};
+            // in this order and no other: LDS is read two operands ahead
+            floatx16 s[2] = {floatx16{}, floatx16{}};
 #pragma unroll
-                for (int i = 0; i < 2 * KS; i++) {
-                    ring[(i + 2) % 4] = operand(i + 2, buffer);
+            for (int i = 0; i < 2 * KS; i++) {
+                ring[(i + 2) % 4] = operand(i + 2, buffer);
 #pragma unroll
-                    for (int term = 0; term < QT; term++)
-                        s[i & 1] = Page<BF>::mfma_wide(ring[i % 4], q[term][i >> 1], s[i & 1]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+                for (int term = 0; term < QT; term++)
+                    s[i & 1] = Page<BF>::mfma_wide(ring[i % 4], q[term][i >> 1], s[i & 1]);
+                __builtin_amdgcn_sched_barrier(0);
             }
             const uint32_t t0 = at_page * kPageTokens;
             if (!(t0 >= u.full0 && t0 + kPageTokens <= u.full1)) {
@@ -682,10 +670,6 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
                 for (int db = 0; db < DB; db++) acc[db] = acc[db] * keep;
             }
             const float from = kLift - (m == -INFINITY ? 0.0f : m);
-            // The next page's scores (the last turn's are of no use), and beside
-            // each product a share of this page's exponentials; then this page's
-            // values by its probabilities.  In this order and no other: LDS is
-            // read two operands ahead of their products.
             float part[2] = {0.0f, 0.0f};
             u32x4 p[4];
             const auto exponentials = [&](int e) {  // pair e of the 16
@@ -695,48 +679,26 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
                 part[1] += x1;
                 p[e >> 2][e & 3] = pack2<T>(x0, x1);
             };
-            if (kAhead) {
-                ahead[0] = ahead[1] = floatx16{};
+            // a quarter of the exponentials, the rest beside the products of the
+            // quarter before
 #pragma unroll
-                for (int i = 0; i < kSteps; i++) {
-                    if (i + 2 < kSteps) ring[(i + 2) % 4] = operand(i + 2, buffer);
-                    if (i < 2 * KS) {
+            for (int e = 0; e < 4; e++) exponentials(e);
 #pragma unroll
-                        for (int term = 0; term < QT; term++)
-                            ahead[i & 1] = Page<BF>::mfma_wide(ring[i % 4], q[term][i >> 1], ahead[i & 1]);
+            for (int i = 2 * KS; i < kSteps; i++) {
+                if (i + 2 < kSteps) ring[(i + 2) % 4] = operand(i + 2, buffer);
+                const int j = i - 2 * KS, db = j % DB, st = j / DB;
+                acc[db] = Page<BF>::mfma_wide(ring[i % 4], p[st], acc[db]);
 #pragma unroll
-                        for (int e = i * 8 / KS; e < (i + 1) * 8 / KS; e++) exponentials(e);
-                    } else {
-                        const int db = (i - 2 * KS) % DB, st = (i - 2 * KS) / DB;
-                        acc[db] = Page<BF>::mfma_wide(ring[i % 4], p[st], acc[db]);
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++) exponentials(e);
-#pragma unroll
-                for (int i = 2 * KS; i < kSteps; i++) {
-                    if (i + 2 < kSteps) ring[(i + 2) % 4] = operand(i + 2, buffer);
-                    const int j = i - 2 * KS, db = j % DB, st = j / DB;
-                    acc[db] = Page<BF>::mfma_wide(ring[i % 4], p[st], acc[db]);
-#pragma unroll
-                    for (int e = 4 + j * 4 / DB; e < 4 + (j + 1) * 4 / DB; e++)
-                        if (e < 16) exponentials(e);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+                for (int e = 4 + j * 4 / DB; e < 4 + (j + 1) * 4 / DB; e++)
+                    if (e < 16) exponentials(e);
+                __builtin_amdgcn_sched_barrier(0);
             }
             l += part[0] + part[1];
-            if (kAhead) {
-                s[0] = ahead[0];
-                s[1] = ahead[1];
-            }
         }
 
         l += __shfl_xor(l, 32, 64);
         // found again here rather than kept in registers all along
-        uint32_t id = threadIdx.x;
-        asm volatile("" : "+v"(id));
+        const uint32_t id = thread_here();
         const uint32_t r1 = (id >> 6) * 32 + (id & 31), half1 = (id >> 5) & 1;
         if (r1 < u.rows) {
             const RowAt to = row_at(c, u.row0 + r1, h);
@@ -745,12 +707,14 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
             for (int db = 0; db < DB; db++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) odd |= db * 32 + 8 * (i >> 2) < (int)hd && !finite(acc[db][i]);
-            if (odd && finite(l)) again[r1] = any_again = 1;
+            if (odd || !finite(l)) again[r1] = any_again = 1;
             const bool direct = u.part == kNoPart;
             const uint64_t slot = (uint64_t)(u.part + r1) * kvh + h;
             if (half1 == 0) {
-                if (!direct) c.part_ml[slot] = float2{m - kLift, l};
-                if (direct && !(l > 0.0f)) *c.bad.word = c.bad.mark;
+                if (!direct)
+                    c.part_ml[slot] = float2{m - kLift, l};
+                else if (l == 0.0f)
+                    *c.bad.word = c.bad.mark;
             }
             const float over = 1.0f / l;
 #pragma unroll
@@ -768,6 +732,232 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
         }
         __syncthreads();
         if (any_again) careful_rows<BF>(c, u, h, NW, again);
+        __syncthreads();
+    }
+}
+
+// Units of heads of more than 256 dims. The waves share the dims: each has a
+// quarter of every key's and value's, so that its queries and results fit its
+// registers, and every key and value goes into one wave's registers once for up
+// to 48 rows (64 do not fit). What the waves have of a block of 32 scores meets in LDS, where
+// each reads all four and adds them in one order: m, sum and probabilities are
+// the same in every wave. Two places in turn, so that one barrier a block is
+// enough. Keys of the next block are asked for before the barrier.
+template <bool BF, int D, int NB, bool EXACT>
+__global__ __launch_bounds__(256) void attn_dims_kernel(AttnCall c, uint32_t cls) {
+    typedef typename Page<BF>::T T;
+    constexpr int kRows = 16 * NB, DW = D / 4, KS = DW / 32, DB = DW / 16;
+    constexpr int QT = EXACT && BF ? 3 : 2, PT = EXACT ? 2 : 1;
+    constexpr float kLift = BF ? 0.0f : 10.0f, kSlack = 5.0f;
+    __shared__ floatx4 scores[2][4][2 * NB][64];
+    __shared__ float row_scale[kRows];
+    __shared__ uint32_t again[kRows], any_again;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t hd = c.kv.head_dim, kvh = c.kv.kv_heads;
+    const PlanHeader &head = head_of(c);
+    const AttnUnit *units = (const AttnUnit *)(c.plan + head.unit_at[cls]);
+    const uint32_t *positions = (const uint32_t *)(c.plan + head.position_at);
+    const uint32_t total = head.unit_count[cls] * kvh;
+
+    for (uint32_t job = blockIdx.x; job < total; job += gridDim.x) {
+        const uint32_t h = job % kvh;
+        const AttnUnit u = units[job / kvh];
+        const uint32_t tid = thread_here(), lane = tid & 63u, n16 = lane & 15u, g = lane >> 4;
+        if (tid < kRows) again[tid] = 0;
+        if (tid == 0) any_again = 0;
+        const uint32_t *table = c.kv.table + (uint64_t)u.seq * c.kv.row;
+        const uint32_t blocks = (u.kv1 + 31) / 32;
+        // keys 16 (g / 2) + 4 (g % 2) + i + 8 a of a block, as in attn_split_kernel
+        const uint32_t key = 16 * (n16 >> 3) + 4 * ((n16 >> 2) & 1) + (n16 & 3);
+        const auto block_at = [&](uint32_t page) {
+            return (const T *)c.kv.base + ((uint64_t)page * kvh + h) * 2 * hd * kPageTokens;
+        };
+        const auto load_keys = [&](u32x4 *k, uint32_t page, uint32_t b) {
+            const T *kl = block_at(page) + ((b & 1) * 32 + key) * 8;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const uint32_t ch = (wave * KS + ks) * 4 + g;
+                k[2 * ks] = k[2 * ks + 1] = u32x4{0, 0, 0, 0};
+                if (ch * 8 < hd) {
+                    k[2 * ks] = *(const u32x4 *)(kl + ch * 512);
+                    k[2 * ks + 1] = *(const u32x4 *)(kl + ch * 512 + 64);
+                }
+            }
+        };
+        uint32_t b = u.kv0 / 32;
+        uint32_t page = word_at(table, b >> 1), page1 = word_at(table, min(b + 1, blocks - 1) >> 1);
+        u32x4 k[2 * KS];
+        load_keys(k, page, b);
+        // ---- queries: the wave's dims of every row ----
+        if (!BF && c.q_type == kF32) {  // F16 terms: rows by a power of two, as in attn_split_kernel
+            constexpr int kPer = 4;
+            const uint32_t r = tid / kPer;
+            const RowAt at = row_at(c, u.row0 + min(r, u.rows - 1), h);
+            float top = 0.0f;
+            for (uint32_t ch = tid % kPer; ch < hd / 8; ch += kPer) {
+                float v[8];
+                load_eight<BF>(c.q, true, at.token * c.q_stride + (uint64_t)at.head * hd + ch * 8, v);
+#pragma unroll
+                for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(v[e]));
+            }
+#pragma unroll
+            for (int e = kPer / 2; e >= 1; e >>= 1) top = fmaxf(top, __shfl_xor(top, e, 64));
+            if (tid % kPer == 0 && r < kRows)
+                row_scale[r] = top > 0.0f && finite(top) ? (float)((int)(__float_as_uint(top) >> 23) - 127 - 14) : 0.0f;
+        } else if (tid < kRows) {
+            row_scale[tid] = 0.0f;
+        }
+        __syncthreads();
+        u32x4 q[QT][NB][KS];
+        float scale[NB];
+        uint32_t lo[NB], hi[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+            const uint32_t r = nb * 16 + n16;
+            const bool there = r < u.rows;
+            const RowAt at = row_at(c, u.row0 + (there ? r : 0), h);
+            const uint64_t q0 = at.token * c.q_stride + (uint64_t)at.head * hd;
+            lo[nb] = 0;
+            hi[nb] = 0xffffffffu;
+            if (there) seen(c, positions[at.token], lo[nb], hi[nb]);
+            const int e = (int)row_scale[r];
+            scale[nb] = ldexpf(c.scale, e);
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const uint32_t ch = (wave * KS + ks) * 4 + g;
+                float v[8];
+                load_eight<BF>(c.q, c.q_type == kF32, q0 + min(ch, hd / 8 - 1) * 8, v);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    v[i] = there && ch * 8 < hd ? v[i] : 0.0f;
+                    if (!BF) v[i] = ldexpf(v[i], -e);
+                }
+#pragma unroll
+                for (int term = 0; term < QT; term++) q[term][nb][ks] = split8<T>(v);
+            }
+            in_order();
+        }
+        floatx4 acc[DB][NB];
+#pragma unroll
+        for (int db = 0; db < DB; db++)
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) acc[db][nb] = floatx4{0, 0, 0, 0};
+        float m[NB], l[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) m[nb] = -INFINITY, l[nb] = 0.0f;
+
+#pragma unroll 1
+        for (; b < blocks; b++) {
+            const T *vp = block_at(page) + hd * kPageTokens + ((b & 1) * 4 + g) * hd * 8;
+            floatx4 s[2][NB];
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) s[0][nb] = s[1][nb] = floatx4{0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int term = 0; term < QT; term++)
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++) {
+                        s[0][nb] = Page<BF>::mfma(k[2 * ks], q[term][nb][ks], s[0][nb]);
+                        s[1][nb] = Page<BF>::mfma(k[2 * ks + 1], q[term][nb][ks], s[1][nb]);
+                    }
+            if (b + 1 < blocks) load_keys(k, page1, b + 1);
+            page = page1;
+            page1 = word_at(table, min(b + 2, blocks - 1) >> 1);
+            floatx4(*put)[64] = scores[b & 1][wave];
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) put[nb][lane] = s[0][nb], put[NB + nb][lane] = s[1][nb];
+            scores_met();
+            u32x4 v[DB];
+#pragma unroll
+            for (int db = 0; db < DB; db++) {
+                const uint32_t d = (wave * DB + db) * 16 + n16;
+                v[db] = *(const u32x4 *)(vp + min(d, hd - 1) * 8);
+            }
+            const uint32_t t0 = b * 32;
+            const bool whole = t0 >= u.full0 && t0 + 32 <= u.full1;
+            u32x4 p[PT][NB];
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) {
+                in_order();
+                float x[8];
+#pragma unroll
+                for (int a = 0; a < 2; a++) {
+                    floatx4 sum = scores[b & 1][0][a * NB + nb][lane];
+#pragma unroll
+                    for (int w = 1; w < 4; w++) sum += scores[b & 1][w][a * NB + nb][lane];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[a * 4 + i] = sum[i] * scale[nb];
+                }
+                if (!whole) {
+                    const uint32_t first = t0 + 16 * (g >> 1) + 4 * (g & 1);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const uint32_t t = first + (i & 3) + 8 * (i >> 2);
+                        x[i] = t >= lo[nb] && t < hi[nb] ? x[i] : -INFINITY;
+                    }
+                }
+                float top = x[0];
+#pragma unroll
+                for (int i = 1; i < 8; i++) top = fmaxf(top, x[i]);
+                if (__any(top > m[nb] + kSlack)) {
+                    top = fmaxf(top, __shfl_xor(top, 16, 64));
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    const float next = fmaxf(m[nb], top);
+                    const float keep = m[nb] == next ? 1.0f : exp2_hw(m[nb] - next);
+                    m[nb] = next;
+                    l[nb] *= keep;
+#pragma unroll
+                    for (int db = 0; db < DB; db++) acc[db][nb] = acc[db][nb] * keep;
+                }
+                const float from = (m[nb] == -INFINITY ? 0.0f : m[nb]) - kLift;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    x[i] = exp2_hw(x[i] - from);
+                    l[nb] += x[i];
+                }
+#pragma unroll
+                for (int term = 0; term < PT; term++) p[term][nb] = split8<T>(x);
+            }
+#pragma unroll
+            for (int db = 0; db < DB; db++)
+#pragma unroll
+                for (int term = 0; term < PT; term++)
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++) acc[db][nb] = Page<BF>::mfma(v[db], p[term][nb], acc[db][nb]);
+        }
+
+        const uint32_t lane1 = thread_here() & 63u, g1 = lane1 >> 4;  // as in attn_tile_kernel
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+            const uint32_t r = nb * 16 + (lane1 & 15);
+            float sum = l[nb] + __shfl_xor(l[nb], 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            if (r >= u.rows) continue;
+            const RowAt at = row_at(c, u.row0 + r, h);
+            const uint64_t slot = (uint64_t)(u.part + r) * kvh + h;
+            bool odd = false;
+#pragma unroll
+            for (int db = 0; db < DB; db++) {
+                const uint32_t d = (wave * DB + db) * 16 + g1 * 4;
+                if (d >= hd) continue;
+                const floatx4 o = acc[db][nb];
+                odd |= !finite(o[0]) || !finite(o[1]) || !finite(o[2]) || !finite(o[3]);
+                if (u.part == kNoPart)
+                    store_four(c.out, c.out_type, at.token * c.out_stride + (uint64_t)at.head * hd + d, o / sum);
+                else
+                    *(f32x4a4 *)(c.part_o + slot * hd + d) = o;
+            }
+            if (odd || !finite(sum)) again[r] = any_again = 1;
+            if (wave == 0 && g1 == 0) {
+                if (u.part != kNoPart)
+                    c.part_ml[slot] = float2{m[nb] - kLift, sum};
+                else if (sum == 0.0f)
+                    *c.bad.word = c.bad.mark;
+            }
+        }
+        __syncthreads();
+        if (any_again) careful_rows<BF>(c, u, h, 4, again);
         __syncthreads();
     }
 }
@@ -807,13 +997,22 @@ __global__ __launch_bounds__(64 * kJoinRows) void attn_join_kernel(AttnCall c) {
                 f = ml.y == 0.0f ? 0.0f : ml.x == top ? 1.0f : exp2_hw(ml.x - top);
                 sum += ml.y * f;
             }
-#pragma unroll 8
-            for (uint32_t i = 0; i < n; i++) {
-                const uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)slot, (int)i);
-                const float w = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(f), (int)i));
-                const floatv v = *(const floatv *)(c.part_o + ((uint64_t)at * kvh + h) * hd + d);
+            for (uint32_t i = 0; i < n; i += 8) {
+                floatv v[8];
+                float w[8];
 #pragma unroll
-                for (int e = 0; e < V; e++) o[e] = __builtin_fmaf(w, v[e], o[e]);
+                for (uint32_t j = 0; j < 8; j++) {  // the last one again, for nothing, behind the end
+                    const uint32_t k = min(i + j, n - 1);
+                    const uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)slot, (int)k);
+                    w[j] = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(f), (int)k));
+                    v[j] = *(const floatv *)(c.part_o + ((uint64_t)at * kvh + h) * hd + d);
+                }
+#pragma unroll
+                for (uint32_t j = 0; j < 8; j++)
+                    if (i + j < n) {
+#pragma unroll
+                        for (int e = 0; e < V; e++) o[e] = __builtin_fmaf(w[j], v[j][e], o[e]);
+                    }
             }
         }
         sum = wave_sum(sum);
@@ -826,23 +1025,29 @@ __global__ __launch_bounds__(64 * kJoinRows) void attn_join_kernel(AttnCall c) {
     }
 }
 
-static constexpr int some_blocks(int d) { return d <= 128 ? 4 : 2; }
+static constexpr int some_blocks(int d) { return d <= 128 ? 4 : d <= 256 ? 2 : 3; }
 
 static constexpr int tile_waves(int d) { return 4; }
 
 uint32_t attn_pages_rows(uint32_t cls, uint32_t head_dim, bool exact) {
     if (cls == 0) return 16;
     if (cls == 2) return exact || head_dim > 256 ? 0 : 32 * tile_waves(head_dim <= 128 ? 128 : 256);
-    if (cls == 1 && head_dim <= 256) return 16 * some_blocks(head_dim <= 128 ? 128 : 256);
-    return 0;
+    return 16 * some_blocks(head_dim <= 128 ? 128 : head_dim <= 256 ? 256 : 512);
 }
 
 template <bool BF, int D, bool EXACT>
 static hipError_t launch_split(hipStream_t s, uint32_t cls, uint32_t grid, const AttnCall &call) {
-    if (cls == 0)
-        attn_split_kernel<BF, D, 1, EXACT><<<grid, 64 * kSplitWaves, 0, s>>>(call, cls);
-    else if constexpr (D <= 256)
-        attn_split_kernel<BF, D, some_blocks(D), EXACT><<<grid, 64 * kSplitWaves, 0, s>>>(call, cls);
+    if constexpr (D > 256) {
+        if (cls == 0)
+            attn_dims_kernel<BF, D, 1, EXACT><<<grid, 256, 0, s>>>(call, cls);
+        else
+            attn_dims_kernel<BF, D, some_blocks(D), EXACT><<<grid, 256, 0, s>>>(call, cls);
+    } else {
+        if (cls == 0)
+            attn_split_kernel<BF, D, 1, EXACT><<<grid, 64 * kSplitWaves, 0, s>>>(call, cls);
+        else
+            attn_split_kernel<BF, D, some_blocks(D), EXACT><<<grid, 64 * kSplitWaves, 0, s>>>(call, cls);
+    }
     return hipGetLastError();
 }
 
