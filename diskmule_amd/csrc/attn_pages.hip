@@ -176,6 +176,13 @@ __device__ __forceinline__ uint32_t word_at(const uint32_t *p, uint32_t i) {
     return ((const __attribute__((address_space(4))) uint32_t *)p)[i];
 }
 
+// F16 terms of a 32-bit query: its row is divided by 2^e, which brings the
+// largest value to 2^14, so that none overflows and the second term of a small
+// one is still there.
+__device__ __forceinline__ int row_power(float largest) {
+    return largest > 0.0f && finite(largest) ? (int)(__float_as_uint(largest) >> 23) - 127 - 14 : 0;
+}
+
 // The positions a query at `position` sees: [lo, hi).
 __device__ __forceinline__ void seen(const AttnCall &c, uint32_t position, uint32_t &lo, uint32_t &hi) {
     hi = position + 1;
@@ -309,29 +316,23 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
             const bool there = r < u.rows;
             const RowAt at = row_at(c, u.row0 + (there ? r : 0), h);
             const uint64_t q0 = at.token * c.q_stride + (uint64_t)at.head * hd;
-            int e = 0;
-            if (!BF && c.q_type == kF32) {
-                // F16 terms of a 32-bit query: its row by a power of two that
-                // brings the largest to 2^14, so that none overflows and the
-                // second half of a small one is still there
-                float top = 0.0f;
-                if (there)
-                    for (uint32_t ch = sub; ch < hd / 8; ch += kPer) {
-                        float v[8];
-                        load_eight<BF>(c.q, true, q0 + ch * 8, v);
-#pragma unroll
-                        for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(v[k]));
-                    }
-#pragma unroll
-                for (int k = kPer / 2; k >= 1; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
-                if (top > 0.0f && finite(top)) e = (int)(__float_as_uint(top) >> 23) - 127 - 14;
-            }
-            if (sub == 0) row_scale[r] = ldexpf(c.scale, e);
             constexpr int kChunks = (D / 8 + kPer - 1) / kPer;  // of a thread
             float all[kChunks][8];
 #pragma unroll
             for (int i = 0; i < kChunks; i++)  // every lane loads, so that the loads go out together
                 load_eight<BF>(c.q, c.q_type == kF32, q0 + min(sub + i * kPer, hd / 8 - 1) * 8, all[i]);
+            int e = 0;
+            if (!BF && c.q_type == kF32) {
+                float top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kChunks; i++)
+#pragma unroll
+                    for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(all[i][k]));
+#pragma unroll
+                for (int k = kPer / 2; k >= 1; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
+                e = row_power(top);
+            }
+            if (sub == 0) row_scale[r] = ldexpf(c.scale, e);
 #pragma unroll
             for (int i = 0; i < kChunks; i++) {
                 const uint32_t ch = sub + i * kPer;
@@ -535,6 +536,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
     constexpr int kHalf = D * kPageTokens * 2;  // bytes of a page's keys in LDS, and of its values
     constexpr float kLift = BF ? 0.0f : 10.0f, kSlack = 5.0f;
     constexpr int kSteps = 2 * KS + 4 * DB;  // products of a page, by their first operand from LDS
+    constexpr int kDeep = D <= 128 ? 4 : 6;
     extern __shared__ __attribute__((aligned(16))) uint8_t stage[];  // keys, keys, values, values
     __shared__ uint32_t again[kRows], any_again;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -582,34 +584,29 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
         float scale = c.scale;
         {
             const uint64_t q0 = at.token * c.q_stride + (uint64_t)at.head * hd;
-            int e = 0;
-            if (!BF && QT == 2) {  // as in attn_split_kernel
-                float top = 0.0f;
-                for (uint32_t ch = half; ch < hd / 8; ch += 2) {
-                    float v[8];
-                    load_eight<BF>(c.q, true, q0 + ch * 8, v);
+            float v[KS][8];
 #pragma unroll
-                    for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(v[k]));
-                }
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
-                if (top > 0.0f && finite(top)) e = (int)(__float_as_uint(top) >> 23) - 127 - 14;
+            for (int s = 0; s < KS; s++)
+                load_eight<BF>(c.q, QT == 2, q0 + min(2 * s + half, hd / 8 - 1) * 8, v[s]);
+            int e = 0;
+            if (!BF && QT == 2) {
+                float top = 0.0f;
+#pragma unroll
+                for (int s = 0; s < KS; s++)
+#pragma unroll
+                    for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(v[s][k]));
+                e = row_power(fmaxf(top, __shfl_xor(top, 32, 64)));
             }
             scale = ldexpf(scale, e);
 #pragma unroll
             for (int s = 0; s < KS; s++) {
-                if (D > 128 || s % 4 == 0) in_order();
-                const uint32_t ch = 2 * s + half;
-                float v[8];
-                // every lane loads, so that the loads go out together
-                load_eight<BF>(c.q, QT == 2, q0 + min(ch, hd / 8 - 1) * 8, v);
 #pragma unroll
-                for (int k = 0; k < 8; k++) v[k] = there && ch * 8 < hd ? v[k] : 0.0f;
-                if (!BF && QT == 2) {
-#pragma unroll
-                    for (int k = 0; k < 8; k++) v[k] = ldexpf(v[k], -e);
+                for (int k = 0; k < 8; k++) {
+                    v[s][k] = there && (2 * s + half) * 8 < hd ? v[s][k] : 0.0f;
+                    if (!BF && QT == 2) v[s][k] = ldexpf(v[s][k], -e);
                 }
 #pragma unroll
-                for (int term = 0; term < QT; term++) q[term][s] = split8<T>(v);
+                for (int term = 0; term < QT; term++) q[term][s] = split8<T>(v[s]);
             }
         }
         floatx16 acc[DB];
@@ -624,7 +621,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
             const int db = (i - 2 * KS) % DB, st = (i - 2 * KS) / DB;
             return *(const u32x4 *)(stage + (2 + buffer) * kHalf + (half * hd + n32) * 16 + (st * 2 * hd + db * 32) * 16);
         };
-        u32x4 ring[4];
+        u32x4 ring[8];
         uint32_t buffer = 0;
 #pragma unroll 1
         for (uint32_t at_page = first; at_page <= last; at_page++, buffer ^= 1) {
@@ -634,16 +631,17 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
                 fetch(page, 1, buffer ^ 1);
             }
             page = word_at(table, min(at_page + 2, last));
-            ring[0] = operand(0, buffer);
-            ring[1] = operand(1, buffer);
-            // in this order and no other: LDS is read two operands ahead
+            if (wave * 32 >= u.rows) continue;  // this wave has no rows
+#pragma unroll
+            for (int i = 0; i < kDeep; i++) ring[i] = operand(i, buffer);
+            // in this order and no other: LDS is read kDeep operands ahead
             floatx16 s[2] = {floatx16{}, floatx16{}};
 #pragma unroll
             for (int i = 0; i < 2 * KS; i++) {
-                ring[(i + 2) % 4] = operand(i + 2, buffer);
+                ring[(i + kDeep) % 8] = operand(i + kDeep, buffer);
 #pragma unroll
                 for (int term = 0; term < QT; term++)
-                    s[i & 1] = Page<BF>::mfma_wide(ring[i % 4], q[term][i >> 1], s[i & 1]);
+                    s[i & 1] = Page<BF>::mfma_wide(ring[i % 8], q[term][i >> 1], s[i & 1]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             const uint32_t t0 = at_page * kPageTokens;
@@ -685,9 +683,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
             for (int e = 0; e < 4; e++) exponentials(e);
 #pragma unroll
             for (int i = 2 * KS; i < kSteps; i++) {
-                if (i + 2 < kSteps) ring[(i + 2) % 4] = operand(i + 2, buffer);
+                if (i + kDeep < kSteps) ring[(i + kDeep) % 8] = operand(i + kDeep, buffer);
                 const int j = i - 2 * KS, db = j % DB, st = j / DB;
-                acc[db] = Page<BF>::mfma_wide(ring[i % 4], p[st], acc[db]);
+                acc[db] = Page<BF>::mfma_wide(ring[i % 8], p[st], acc[db]);
 #pragma unroll
                 for (int e = 4 + j * 4 / DB; e < 4 + (j + 1) * 4 / DB; e++)
                     if (e < 16) exponentials(e);
@@ -750,7 +748,7 @@ __global__ __launch_bounds__(256) void attn_dims_kernel(AttnCall c, uint32_t cls
     constexpr int QT = EXACT && BF ? 3 : 2, PT = EXACT ? 2 : 1;
     constexpr float kLift = BF ? 0.0f : 10.0f, kSlack = 5.0f;
     __shared__ floatx4 scores[2][4][2 * NB][64];
-    __shared__ float row_scale[kRows];
+    __shared__ float row_top[4][kRows];
     __shared__ uint32_t again[kRows], any_again;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t hd = c.kv.head_dim, kvh = c.kv.kv_heads;
@@ -789,53 +787,56 @@ __global__ __launch_bounds__(256) void attn_dims_kernel(AttnCall c, uint32_t cls
         u32x4 k[2 * KS];
         load_keys(k, page, b);
         // ---- queries: the wave's dims of every row ----
-        if (!BF && c.q_type == kF32) {  // F16 terms: rows by a power of two, as in attn_split_kernel
-            constexpr int kPer = 4;
-            const uint32_t r = tid / kPer;
-            const RowAt at = row_at(c, u.row0 + min(r, u.rows - 1), h);
-            float top = 0.0f;
-            for (uint32_t ch = tid % kPer; ch < hd / 8; ch += kPer) {
-                float v[8];
-                load_eight<BF>(c.q, true, at.token * c.q_stride + (uint64_t)at.head * hd + ch * 8, v);
-#pragma unroll
-                for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(v[e]));
-            }
-#pragma unroll
-            for (int e = kPer / 2; e >= 1; e >>= 1) top = fmaxf(top, __shfl_xor(top, e, 64));
-            if (tid % kPer == 0 && r < kRows)
-                row_scale[r] = top > 0.0f && finite(top) ? (float)((int)(__float_as_uint(top) >> 23) - 127 - 14) : 0.0f;
-        } else if (tid < kRows) {
-            row_scale[tid] = 0.0f;
-        }
-        __syncthreads();
         u32x4 q[QT][NB][KS];
         float scale[NB];
         uint32_t lo[NB], hi[NB];
+        {
+            float v[NB][KS][8];
 #pragma unroll
-        for (int nb = 0; nb < NB; nb++) {
-            const uint32_t r = nb * 16 + n16;
-            const bool there = r < u.rows;
-            const RowAt at = row_at(c, u.row0 + (there ? r : 0), h);
-            const uint64_t q0 = at.token * c.q_stride + (uint64_t)at.head * hd;
-            lo[nb] = 0;
-            hi[nb] = 0xffffffffu;
-            if (there) seen(c, positions[at.token], lo[nb], hi[nb]);
-            const int e = (int)row_scale[r];
-            scale[nb] = ldexpf(c.scale, e);
+            for (int nb = 0; nb < NB; nb++) {
+                const uint32_t r = nb * 16 + n16;
+                const bool there = r < u.rows;
+                const RowAt at = row_at(c, u.row0 + (there ? r : 0), h);
+                const uint64_t q0 = at.token * c.q_stride + (uint64_t)at.head * hd;
+                lo[nb] = 0;
+                hi[nb] = 0xffffffffu;
+                if (there) seen(c, positions[at.token], lo[nb], hi[nb]);
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                const uint32_t ch = (wave * KS + ks) * 4 + g;
-                float v[8];
-                load_eight<BF>(c.q, c.q_type == kF32, q0 + min(ch, hd / 8 - 1) * 8, v);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    v[i] = there && ch * 8 < hd ? v[i] : 0.0f;
-                    if (!BF) v[i] = ldexpf(v[i], -e);
-                }
-#pragma unroll
-                for (int term = 0; term < QT; term++) q[term][nb][ks] = split8<T>(v);
+                for (int ks = 0; ks < KS; ks++)
+                    load_eight<BF>(c.q, c.q_type == kF32, q0 + min((wave * KS + ks) * 4 + g, hd / 8 - 1) * 8, v[nb][ks]);
             }
-            in_order();
+            if (!BF) {
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                        for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[nb][ks][i]));
+                    top = fmaxf(top, __shfl_xor(top, 16, 64));
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    if (g == 0) row_top[wave][nb * 16 + n16] = top;
+                }
+                __syncthreads();
+            }
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) {
+                const uint32_t r = nb * 16 + n16;
+                int e = 0;
+                if (!BF && c.q_type == kF32)
+                    e = row_power(fmaxf(fmaxf(row_top[0][r], row_top[1][r]), fmaxf(row_top[2][r], row_top[3][r])));
+                scale[nb] = ldexpf(c.scale, e);
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        v[nb][ks][i] = r < u.rows && ((wave * KS + ks) * 4 + g) * 8 < hd ? v[nb][ks][i] : 0.0f;
+                        if (!BF) v[nb][ks][i] = ldexpf(v[nb][ks][i], -e);
+                    }
+#pragma unroll
+                    for (int term = 0; term < QT; term++) q[term][nb][ks] = split8<T>(v[nb][ks]);
+                }
+            }
         }
         floatx4 acc[DB][NB];
 #pragma unroll
@@ -962,12 +963,15 @@ __global__ __launch_bounds__(256) void attn_dims_kernel(AttnCall c, uint32_t cls
     }
 }
 
-// Rows whose positions were shared out: one wave a row, a lane V dims of it. A
-// lane first takes a part's m and sum, 64 parts at once, and then hands the
-// part's weight to all, so that the loads of the parts' o wait for nothing.
+// Rows whose positions were shared out: a wave a row, or the waves of a
+// workgroup a row of many parts; a lane V dims of it. A lane first takes a
+// part's m and sum, 64 parts at once, and then hands the part's weight to all,
+// so that the loads of the parts' o wait for nothing. Bound by the latency of
+// those three loads one after another where there are few rows, else by memory.
 template <int V>
 __global__ __launch_bounds__(64 * kJoinRows) void attn_join_kernel(AttnCall c) {
     typedef float floatv __attribute__((ext_vector_type(V), aligned(4)));
+    __shared__ float meet[kJoinRows][64 * V + 1];
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t hd = c.kv.head_dim, kvh = c.kv.kv_heads;
@@ -979,19 +983,24 @@ __global__ __launch_bounds__(64 * kJoinRows) void attn_join_kernel(AttnCall c) {
     for (uint32_t job = blockIdx.x; job < total; job += gridDim.x) {
         const uint32_t h = job % kvh;
         const JoinItem it = items[job / kvh];
-        if (wave >= it.rows) continue;
-        const uint32_t r = it.row0 + wave;
+        const bool together = it.rows == 1;
+        if (!together && wave >= it.rows) continue;
+        const uint32_t r = it.row0 + (together ? 0 : wave);
         float top = -INFINITY;
         for (uint32_t i = lane; i < it.count; i += 64)
             top = fmaxf(top, c.part_ml[(uint64_t)(parts[it.first + i] + r) * kvh + h].x);
         top = wave_max(top);
         float sum = 0.0f;
         floatv o = 0.0f;
-        for (uint32_t i0 = 0; i0 < it.count; i0 += 64) {
-            const uint32_t n = min(64u, it.count - i0);
-            const uint32_t slot = lane < n ? parts[it.first + i0 + lane] + r : 0;
+        // this wave's parts: first + step * k
+        const uint32_t step = together ? kJoinRows : 1, first = together ? wave : 0;
+        const uint32_t mine = it.count > first ? (it.count - first + step - 1) / step : 0;
+        for (uint32_t k0 = 0; k0 < mine; k0 += 64) {
+            const uint32_t n = min(64u, mine - k0);
+            uint32_t slot = 0;
             float f = 0.0f;
             if (lane < n) {
+                slot = parts[it.first + first + step * (k0 + lane)] + r;
                 const float2 ml = c.part_ml[(uint64_t)slot * kvh + h];
                 // a part that saw nothing has no weight, whatever m is
                 f = ml.y == 0.0f ? 0.0f : ml.x == top ? 1.0f : exp2_hw(ml.x - top);
@@ -1016,12 +1025,29 @@ __global__ __launch_bounds__(64 * kJoinRows) void attn_join_kernel(AttnCall c) {
             }
         }
         sum = wave_sum(sum);
-        if (lane == 0 && !(sum > 0.0f)) *c.bad.word = c.bad.mark;
-        const RowAt at = row_at(c, r, h);
-        const uint64_t to = at.token * c.out_stride + (uint64_t)at.head * hd + lane * V;
-        if (lane * V < hd)
+        if (together) {
 #pragma unroll
-            for (int e = 0; e < V; e += 2) store_two(c.out, c.out_type, to + e, o[e] / sum, o[e + 1] / sum);
+            for (int e = 0; e < V; e++) meet[wave][lane * V + e] = o[e];
+            if (lane == 0) meet[wave][64 * V] = sum;
+            __syncthreads();
+            sum = 0.0f;
+            o = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < kJoinRows; w++) {
+                sum += meet[w][64 * V];
+#pragma unroll
+                for (int e = 0; e < V; e++) o[e] += meet[w][lane * V + e];
+            }
+            __syncthreads();
+        }
+        if (!together || wave == 0) {
+            if (lane == 0 && !(sum > 0.0f)) *c.bad.word = c.bad.mark;
+            const RowAt at = row_at(c, r, h);
+            const uint64_t to = at.token * c.out_stride + (uint64_t)at.head * hd + lane * V;
+            if (lane * V < hd)
+#pragma unroll
+                for (int e = 0; e < V; e += 2) store_two(c.out, c.out_type, to + e, o[e] / sum, o[e + 1] / sum);
+        }
     }
 }
 
@@ -1033,6 +1059,13 @@ uint32_t attn_pages_rows(uint32_t cls, uint32_t head_dim, bool exact) {
     if (cls == 0) return 16;
     if (cls == 2) return exact || head_dim > 256 ? 0 : 32 * tile_waves(head_dim <= 128 ? 128 : 256);
     return 16 * some_blocks(head_dim <= 128 ? 128 : head_dim <= 256 ? 256 : 512);
+}
+
+// By their registers and LDS, which the build reports.
+uint32_t attn_pages_resident(uint32_t cls, uint32_t head_dim) {
+    if (cls == 0) return 2;
+    if (cls == 1) return head_dim <= 64 ? 2 : 1;
+    return head_dim <= 128 ? 2 : 1;
 }
 
 template <bool BF, int D, bool EXACT>

@@ -309,8 +309,10 @@ struct AttnUnit {
     uint32_t row0, rows, seq, kv0, kv1, full0, full1, part;
 };
 // Up to kJoinRows rows whose result is joined from `count` partial results: that
-// of row r in part i stands at parts[first + i] + r (modulo 2^32).
-constexpr uint32_t kJoinRows = 4;
+// of row r in part i stands at parts[first + i] + r (modulo 2^32).  A workgroup
+// takes an item with a wave a row, or one row with all its waves, which rows of
+// many parts are given.
+constexpr uint32_t kJoinRows = 4, kManyParts = 8;
 struct JoinItem {
     uint32_t row0, rows, first, count;
 };
@@ -396,9 +398,9 @@ class Planner {
     };
     // Units over one range of positions for the rows of sequences lo .. hi - 1.
     struct Level {
-        uint32_t row0, rows, seq, cls, tile;
-        uint64_t kv0, kv1;
-        size_t lo, hi;
+        uint32_t row0 = 0, rows = 0, seq = 0, cls = 0, tile = 0;
+        uint64_t kv0 = 0, kv1 = 0;
+        size_t lo = 0, hi = 0;
         std::vector<std::vector<uint32_t>> parts;  // of each row tile
     };
 
@@ -416,6 +418,13 @@ class Planner {
         paths_.clear();
         std::vector<size_t> path;
         split(0, items_.size(), 0, path);
+        // one launch for all: of the kernel that the most rows need
+        uint32_t cls = 0;
+        for (const Level &l : levels_) cls = std::max(cls, class_of(l.rows));
+        for (Level &l : levels_) {
+            l.cls = cls;
+            l.tile = shape_.rows_of[cls];
+        }
         // positions that the units of each class go through, which decide how
         // long one of them may be
         uint64_t work[kUnitClasses] = {};
@@ -474,16 +483,19 @@ class Planner {
         l.row0 = items_[lo].token0 * shape_.group;
         l.rows = (last.token0 + last.count) * shape_.group - l.row0;
         l.seq = items_[lo].seq;
-        // the smallest kernel that takes all rows in one unit, else the largest there is
-        l.cls = 0;
-        while (l.cls + 1 < kUnitClasses && shape_.rows_of[l.cls + 1] && l.rows > shape_.rows_of[l.cls]) l.cls++;
-        l.tile = shape_.rows_of[l.cls];
         l.kv0 = kv0;
         l.kv1 = kv1;
         l.lo = lo;
         l.hi = hi;
         levels_.push_back(l);
         return levels_.size() - 1;
+    }
+
+    // The smallest kernel that takes all rows in one unit, else the largest there is.
+    uint32_t class_of(uint32_t rows) const {
+        uint32_t cls = 0;
+        while (cls + 1 < kUnitClasses && shape_.rows_of[cls + 1] && rows > shape_.rows_of[cls]) cls++;
+        return cls;
     }
 
     uint32_t position(uint32_t row) const { return out_->positions[row / shape_.group]; }
@@ -524,9 +536,9 @@ class Planner {
             range(*l, r, &a, &b);
             bounds(*l, r, &low, &high);
             if (a == b) continue;
-            // even chunks of whole pages
+            // even chunks of whole pages, as many as come nearest to the wanted length
             const uint64_t pages = (b - a + kPageTokens - 1) / kPageTokens;
-            uint64_t n = plain_ ? 1 : std::min(pages, (b - a + chunk_[l->cls] - 1) / chunk_[l->cls]);
+            const uint64_t n = plain_ ? 1 : std::max<uint64_t>(1, std::min(pages, (b - a + chunk_[l->cls] / 2) / chunk_[l->cls]));
             const bool direct = alone && n == 1;
             const uint64_t full0 = shape_.window && high + 1ull > shape_.window ? high + 1 - shape_.window : 0;
             for (uint64_t i = 0; i < n; i++) {
@@ -573,8 +585,10 @@ class Planner {
             item.count = (uint32_t)out_->parts.size() - item.first;
             const uint32_t to = r + item.rows;
             if (item.count)  // none: the one unit wrote its rows itself
-                for (uint32_t a = r; a < to; a += kJoinRows)
-                    out_->joins.push_back({a, std::min(kJoinRows, to - a), item.first, item.count});
+                for (uint32_t a = r, rows; a < to; a += rows) {
+                    rows = item.count >= kManyParts ? 1 : std::min(kJoinRows, to - a);
+                    out_->joins.push_back({a, rows, item.first, item.count});
+                }
             r = to;
             if (!plain_ && !fits()) return false;
         }

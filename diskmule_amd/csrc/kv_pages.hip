@@ -540,12 +540,12 @@ int dmhip_new_kv_plan(dmhip_kv_pages *pool, size_t query_heads, int has_window, 
     uint32_t most = 0;
     for (uint32_t c = 0; c < kUnitClasses; c++) {
         s.rows_of[c] = attn_pages_rows(c, pool->head_dim, output_type == kF32);
-        s.workgroups[c] = 2 * cus;
+        s.workgroups[c] = attn_pages_resident(c, pool->head_dim) * cus;
         most = std::max(most, s.rows_of[c]);
     }
     const size_t sequences = std::min<size_t>(pool->book.sequences(), max_tokens);
     s.max_parts = 2 * std::min(rows, sequences * kSharedRows) + 4 * (size_t)cus * most / pool->kv_heads + most;
-    s.max_bytes = plan_least_bytes(max_tokens, group, sequences) + rows / kJoinRows * sizeof(JoinItem) + (512u << 10);
+    s.max_bytes = plan_least_bytes(max_tokens, group, sequences) + std::min(rows, s.max_parts / 2) * sizeof(JoinItem) + (512u << 10);
     p->list_bytes = sizeof(PlanHeader) + s.max_bytes + 16 * 8;
     const size_t part_rows = s.max_parts * pool->kv_heads;
     const size_t sizes[3] = {p->list_bytes, part_rows * pool->head_dim * 4, part_rows * sizeof(float2)};
