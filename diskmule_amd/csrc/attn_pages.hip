@@ -197,7 +197,21 @@ __device__ __forceinline__ RowAt row_at(const AttnCall &c, uint32_t row, uint32_
     return {t, h * c.group + (row - t * c.group)};
 }
 
-__device__ __forceinline__ const PlanHeader &head_of(const AttnCall &c) { return *(const PlanHeader *)c.plan; }
+// The units of a class. A captured launch reads the plan's head where it is, so
+// that it works on what the plan holds when it is replayed.
+struct UnitList {
+    const AttnUnit *units;
+    const uint32_t *positions;
+    uint32_t count;
+};
+template <uint32_t CLS>
+__device__ __forceinline__ UnitList units_of(const AttnCall &c) {
+    const auto from = [&](const PlanHeader &h) {
+        return UnitList{(const AttnUnit *)(c.plan + h.unit_at[CLS]), (const uint32_t *)(c.plan + h.position_at),
+                        h.unit_count[CLS]};
+    };
+    return c.captured ? from(*(const PlanHeader *)c.plan) : from(c.head);
+}
 
 // Rows of a unit again, with every masked product left out instead of
 // multiplied by zero, and queries and probabilities in 32 bits: for rows whose
@@ -206,11 +220,11 @@ __device__ __forceinline__ const PlanHeader &head_of(const AttnCall &c) { return
 // one that it does see gives inf - inf where queries or probabilities are split
 // into several values. One wave a row: a lane a key, then a lane a dim.
 template <bool BF>
-__device__ void careful_rows(const AttnCall &c, const AttnUnit &u, uint32_t h, uint32_t waves, const uint32_t *again) {
+__device__ void careful_rows(const AttnCall &c, const AttnUnit &u, uint32_t h, uint32_t waves, const uint32_t *again,
+                             const uint32_t *positions) {
     typedef typename Page<BF>::T T;
     const uint32_t lane = thread_here() & 63u;
     const uint32_t hd = c.kv.head_dim;
-    const uint32_t *positions = (const uint32_t *)(c.plan + head_of(c).position_at);
     for (uint32_t r = threadIdx.x >> 6; r < u.rows; r += waves) {
         if (!again[r]) continue;
         const RowAt at = row_at(c, u.row0 + r, h);
@@ -282,14 +296,16 @@ __device__ void careful_rows(const AttnCall &c, const AttnUnit &u, uint32_t h, u
 // of it, as the result is; a 32-bit query's own rounding would be more, its
 // error being that of the whole score.
 template <bool BF, int D, int NB, bool EXACT>
-__global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c, uint32_t cls) {
+__global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c) {
+    constexpr uint32_t kClass = NB == 1 ? 0 : 1;
     typedef typename Page<BF>::T T;
     constexpr int kRows = 16 * NB, KS = D / 32, DB = D / 16;
     constexpr int QT = EXACT && BF ? 3 : 2, PT = EXACT ? 2 : 1;
     // Probabilities of F16 pages are 2^10 times larger: its smallest value 2^-24
     // would lose the many small ones of a long row.
     constexpr float kLift = BF ? 0.0f : 10.0f;
-    constexpr int kReducePitch = 36;  // floats of a row of 32 dims: rows start 4 banks apart
+    constexpr int kMeet = NB == 1 ? (D < 128 ? D : 128) : 64;  // dims of which the waves' results meet at a time
+    constexpr int kReducePitch = kMeet + 4;                    // floats of a row: rows start 4 banks apart
     constexpr int kQueryBytes = QT * NB * KS * 64 * 16;
     constexpr int kReduceBytes = kSplitWaves * kRows * kReducePitch * 4;
     __shared__ __attribute__((aligned(16))) uint8_t shared[kQueryBytes > kReduceBytes ? kQueryBytes : kReduceBytes];
@@ -298,10 +314,10 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
     __shared__ uint32_t again[kRows], any_again;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t hd = c.kv.head_dim, kvh = c.kv.kv_heads;
-    const PlanHeader &head = head_of(c);
-    const AttnUnit *units = (const AttnUnit *)(c.plan + head.unit_at[cls]);
-    const uint32_t *positions = (const uint32_t *)(c.plan + head.position_at);
-    const uint32_t total = head.unit_count[cls] * kvh;
+    const UnitList list = units_of<kClass>(c);
+    const AttnUnit *units = list.units;
+    const uint32_t *positions = list.positions;
+    const uint32_t total = list.count * kvh;
 
     for (uint32_t job = blockIdx.x; job < total; job += gridDim.x) {
         const uint32_t h = job % kvh;
@@ -309,6 +325,30 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
         const uint32_t tid = thread_here(), lane = tid & 63u, n16 = lane & 15u, g = lane >> 4;
         if (tid < kRows) again[tid] = 0;
         if (tid == 0) any_again = 0;
+        const uint32_t *table = c.kv.table + (uint64_t)u.seq * c.kv.row;
+        const uint32_t blocks = (u.kv1 + 31) / 32, first = u.kv0 / 32 + wave;
+        const auto block_at = [&](uint32_t page) {
+            return (const T *)c.kv.base + ((uint64_t)page * kvh + h) * 2 * hd * kPageTokens;
+        };
+        // Keys of a block: row 4 g + i of half a of its scores is key
+        // 16 (g / 2) + 4 (g % 2) + i + 8 a, so that a lane's eight scores are the
+        // tokens of one value chunk, in its order.
+        const auto load_keys = [&](u32x4 *k, uint32_t page, uint32_t b) {
+            const T *kl = block_at(page) + ((b & 1) * 32 + 16 * (n16 >> 3) + 4 * ((n16 >> 2) & 1) + (n16 & 3)) * 8;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                // every lane loads; dims that the pages do not hold are zero
+                const uint32_t ch = ks * 4 + g, at = min(ch, hd / 8 - 1) * 512;
+                const u32x4 none = {0, 0, 0, 0}, a = *(const u32x4 *)(kl + at), b = *(const u32x4 *)(kl + at + 64);
+                k[2 * ks] = ch * 8 < hd ? a : none;
+                k[2 * ks + 1] = ch * 8 < hd ? b : none;
+            }
+        };
+        uint32_t page = word_at(table, min(first, blocks - 1) >> 1);
+        uint32_t page1 = word_at(table, min(first + kSplitWaves, blocks - 1) >> 1);
+        u32x4 k[2 * KS];
+        load_keys(k, page, min(first, blocks - 1));
+        in_order();
         // ---- queries into LDS, as the B operands of the products ----
         {
             constexpr int kPer = 64 * kSplitWaves / kRows;  // threads of a row, in one wave
@@ -318,9 +358,15 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
             const uint64_t q0 = at.token * c.q_stride + (uint64_t)at.head * hd;
             constexpr int kChunks = (D / 8 + kPer - 1) / kPer;  // of a thread
             float all[kChunks][8];
+            const auto load = [&](bool f32) {  // every lane loads, so that the loads go out together
 #pragma unroll
-            for (int i = 0; i < kChunks; i++)  // every lane loads, so that the loads go out together
-                load_eight<BF>(c.q, c.q_type == kF32, q0 + min(sub + i * kPer, hd / 8 - 1) * 8, all[i]);
+                for (int i = 0; i < kChunks; i++)
+                    load_eight<BF>(c.q, f32, q0 + min(sub + i * kPer, hd / 8 - 1) * 8, all[i]);
+            };
+            if (c.q_type == kF32)
+                load(true);
+            else
+                load(false);
             int e = 0;
             if (!BF && c.q_type == kF32) {
                 float top = 0.0f;
@@ -372,39 +418,34 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) m[nb] = -INFINITY, l[nb] = 0.0f;
 
-        const uint32_t *table = c.kv.table + (uint64_t)u.seq * c.kv.row;
-        const uint32_t blocks = (u.kv1 + 31) / 32;
-        uint32_t page = word_at(table, min(u.kv0 / 32 + wave, blocks - 1) >> 1);  // a block ahead
 #pragma unroll 1
-        for (uint32_t b = u.kv0 / 32 + wave; b < blocks; b += kSplitWaves) {
-            const T *kp = (const T *)c.kv.base + ((uint64_t)page * kvh + h) * 2 * hd * kPageTokens;
-            page = word_at(table, min(b + kSplitWaves, blocks - 1) >> 1);
-            const T *vp = kp + hd * kPageTokens + ((b & 1) * 4 + g) * hd * 8;
-            // Scores of 32 keys: row 4 g + i of half a is key
-            // 16 (g / 2) + 4 (g % 2) + i + 8 a, so that a lane's eight are the
-            // tokens of one value chunk, in its order.
-            const T *kl = kp + ((b & 1) * 32 + 16 * (n16 >> 3) + 4 * ((n16 >> 2) & 1) + (n16 & 3)) * 8;
+        for (uint32_t b = first; b < blocks; b += kSplitWaves) {
+            // values of this block, then its scores, then keys of the next one:
+            // what the memory has to bring is always asked for a step before
+            u32x4 v[DB];
+            const T *vp = block_at(page) + hd * kPageTokens + ((b & 1) * 4 + g) * hd * 8;
+#pragma unroll
+            for (int db = 0; db < DB; db++) v[db] = *(const u32x4 *)(vp + min(db * 16 + n16, hd - 1) * 8);
+            in_order();
             floatx4 s[2][NB];
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) s[0][nb] = s[1][nb] = floatx4{0, 0, 0, 0};
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                if (ks % 4 == 0) in_order();
-                const uint32_t ch = ks * 4 + g;
-                u32x4 k0 = {0, 0, 0, 0}, k1 = {0, 0, 0, 0};
-                if (ch * 8 < hd) {
-                    k0 = *(const u32x4 *)(kl + ch * 512);
-                    k1 = *(const u32x4 *)(kl + ch * 512 + 64);
-                }
+            for (int ks = 0; ks < KS; ks++)
 #pragma unroll
                 for (int term = 0; term < QT; term++)
 #pragma unroll
                     for (int nb = 0; nb < NB; nb++) {
                         const u32x4 q = *(const u32x4 *)(shared + (((term * NB + nb) * KS + ks) * 64 + lane) * 16);
-                        s[0][nb] = Page<BF>::mfma(k0, q, s[0][nb]);
-                        s[1][nb] = Page<BF>::mfma(k1, q, s[1][nb]);
+                        s[0][nb] = Page<BF>::mfma(k[2 * ks], q, s[0][nb]);
+                        s[1][nb] = Page<BF>::mfma(k[2 * ks + 1], q, s[1][nb]);
                     }
+            page = page1;
+            if (b + kSplitWaves < blocks) {
+                load_keys(k, page, b + kSplitWaves);
+                page1 = word_at(table, min(b + 2 * kSplitWaves, blocks - 1) >> 1);
             }
+            in_order();
             const uint32_t t0 = b * 32;
             u32x4 p[PT][NB];
             const bool whole = t0 >= u.full0 && t0 + 32 <= u.full1;
@@ -447,15 +488,11 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
                 for (int term = 0; term < PT; term++) p[term][nb] = split8<T>(x);
             }
 #pragma unroll
-            for (int db = 0; db < DB; db++) {
-                if (db % 8 == 0) in_order();
-                const uint32_t d = db * 16 + n16;
-                const u32x4 v = *(const u32x4 *)(vp + (d < hd ? d : hd - 1) * 8);
+            for (int db = 0; db < DB; db++)
 #pragma unroll
                 for (int term = 0; term < PT; term++)
 #pragma unroll
-                    for (int nb = 0; nb < NB; nb++) acc[db][nb] = Page<BF>::mfma(v, p[term][nb], acc[db][nb]);
-            }
+                    for (int nb = 0; nb < NB; nb++) acc[db][nb] = Page<BF>::mfma(v[db], p[term][nb], acc[db][nb]);
         }
 
         // ---- the waves' results to one m, added ----
@@ -477,17 +514,17 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
         }
         float *reduce = (float *)shared;
 #pragma unroll
-        for (int dc = 0; dc < D / 32; dc++) {
+        for (int dc = 0; dc < D / kMeet; dc++) {
             if (dc) __syncthreads();
 #pragma unroll
             for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-                for (int k = 0; k < 2; k++)
+                for (int k = 0; k < kMeet / 16; k++)
                     *(floatx4 *)(reduce + (wave * kRows + nb * 16 + n16) * kReducePitch + k * 16 + g * 4) =
-                        acc[dc * 2 + k][nb];
+                        acc[dc * (kMeet / 16) + k][nb];
             __syncthreads();
-            for (uint32_t i = tid; i < kRows * 8; i += 64 * kSplitWaves) {
-                const uint32_t r = i >> 3, d = dc * 32 + (i & 7) * 4;
+            for (uint32_t i = tid; i < kRows * kMeet / 4; i += 64 * kSplitWaves) {
+                const uint32_t r = i / (kMeet / 4), at4 = i % (kMeet / 4) * 4, d = dc * kMeet + at4;
                 if (r >= u.rows || d >= hd) continue;
                 float top = -INFINITY, sum = 0.0f;
 #pragma unroll
@@ -500,7 +537,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
                 floatx4 o = {0, 0, 0, 0};
 #pragma unroll
                 for (uint32_t w = 0; w < kSplitWaves; w++)
-                    o += *(const floatx4 *)(reduce + (w * kRows + r) * kReducePitch + (i & 7) * 4);
+                    o += *(const floatx4 *)(reduce + (w * kRows + r) * kReducePitch + at4);
                 const bool odd = !finite(o[0]) || !finite(o[1]) || !finite(o[2]) || !finite(o[3]);
                 if (odd || !finite(sum)) again[r] = any_again = 1;
                 const RowAt at = row_at(c, u.row0 + r, h);
@@ -515,7 +552,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
             }
         }
         __syncthreads();
-        if (any_again) careful_rows<BF>(c, u, h, kSplitWaves, again);
+        if (any_again) careful_rows<BF>(c, u, h, kSplitWaves, again, positions);
         __syncthreads();
     }
 }
@@ -527,10 +564,11 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
 // tokens, so that probabilities go from the scores' registers into the second
 // product as they are, and m and the sum are one number a lane.
 //
-// QT: values of the page type that a query is split into (two for a 32-bit
-// query, whose rounding would be the largest error of the result).
+// QT: values of the page type that a query is split into (two for most 32-bit
+// queries, whose rounding would be the largest error of the result).
 template <bool BF, int D, int QT, int NW>
-__global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(AttnCall c, uint32_t cls) {
+__global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(AttnCall c) {
+    constexpr uint32_t kClass = 2;
     typedef typename Page<BF>::T T;
     constexpr int kRows = 32 * NW, KS = D / 16, DB = D / 32;
     constexpr int kHalf = D * kPageTokens * 2;  // bytes of a page's keys in LDS, and of its values
@@ -541,10 +579,10 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
     __shared__ uint32_t again[kRows], any_again;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t hd = c.kv.head_dim, kvh = c.kv.kv_heads;
-    const PlanHeader &head = head_of(c);
-    const AttnUnit *units = (const AttnUnit *)(c.plan + head.unit_at[cls]);
-    const uint32_t *positions = (const uint32_t *)(c.plan + head.position_at);
-    const uint32_t total = head.unit_count[cls] * kvh;
+    const UnitList list = units_of<kClass>(c);
+    const AttnUnit *units = list.units;
+    const uint32_t *positions = list.positions;
+    const uint32_t total = list.count * kvh;
     // key dims that the pages do not hold are zero for good: no page is copied there
     for (uint32_t i = hd * kPageTokens * 2 + threadIdx.x * 16; i < (uint32_t)kHalf; i += 64 * NW * 16)
         *(u32x4 *)(stage + i) = *(u32x4 *)(stage + kHalf + i) = u32x4{0, 0, 0, 0};
@@ -585,11 +623,16 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
         {
             const uint64_t q0 = at.token * c.q_stride + (uint64_t)at.head * hd;
             float v[KS][8];
+            const auto load = [&](bool f32) {
 #pragma unroll
-            for (int s = 0; s < KS; s++)
-                load_eight<BF>(c.q, QT == 2, q0 + min(2 * s + half, hd / 8 - 1) * 8, v[s]);
+                for (int s = 0; s < KS; s++) load_eight<BF>(c.q, f32, q0 + min(2 * s + half, hd / 8 - 1) * 8, v[s]);
+            };
+            if (QT == 2 || c.q_type == kF32)
+                load(true);
+            else
+                load(false);
             int e = 0;
-            if (!BF && QT == 2) {
+            if (!BF && c.q_type == kF32) {
                 float top = 0.0f;
 #pragma unroll
                 for (int s = 0; s < KS; s++)
@@ -603,7 +646,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
                     v[s][k] = there && (2 * s + half) * 8 < hd ? v[s][k] : 0.0f;
-                    if (!BF && QT == 2) v[s][k] = ldexpf(v[s][k], -e);
+                    if (!BF) v[s][k] = ldexpf(v[s][k], -e);
                 }
 #pragma unroll
                 for (int term = 0; term < QT; term++) q[term][s] = split8<T>(v[s]);
@@ -636,6 +679,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
             for (int i = 0; i < kDeep; i++) ring[i] = operand(i, buffer);
             // in this order and no other: LDS is read kDeep operands ahead
             floatx16 s[2] = {floatx16{}, floatx16{}};
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int i = 0; i < 2 * KS; i++) {
                 ring[(i + kDeep) % 8] = operand(i + kDeep, buffer);
@@ -644,6 +688,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
                     s[i & 1] = Page<BF>::mfma_wide(ring[i % 8], q[term][i >> 1], s[i & 1]);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            __builtin_amdgcn_s_setprio(0);
             const uint32_t t0 = at_page * kPageTokens;
             if (!(t0 >= u.full0 && t0 + kPageTokens <= u.full1)) {
 #pragma unroll
@@ -681,6 +726,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
             // quarter before
 #pragma unroll
             for (int e = 0; e < 4; e++) exponentials(e);
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int i = 2 * KS; i < kSteps; i++) {
                 if (i + kDeep < kSteps) ring[(i + kDeep) % 8] = operand(i + kDeep, buffer);
@@ -691,6 +737,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
                     if (e < 16) exponentials(e);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            __builtin_amdgcn_s_setprio(0);
             l += part[0] + part[1];
         }
 
@@ -729,7 +776,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
                 }
         }
         __syncthreads();
-        if (any_again) careful_rows<BF>(c, u, h, NW, again);
+        if (any_again) careful_rows<BF>(c, u, h, NW, again, positions);
         __syncthreads();
     }
 }
@@ -742,7 +789,8 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
 // the same in every wave. Two places in turn, so that one barrier a block is
 // enough. Keys of the next block are asked for before the barrier.
 template <bool BF, int D, int NB, bool EXACT>
-__global__ __launch_bounds__(256) void attn_dims_kernel(AttnCall c, uint32_t cls) {
+__global__ __launch_bounds__(256) void attn_dims_kernel(AttnCall c) {
+    constexpr uint32_t kClass = NB == 1 ? 0 : 1;
     typedef typename Page<BF>::T T;
     constexpr int kRows = 16 * NB, DW = D / 4, KS = DW / 32, DB = DW / 16;
     constexpr int QT = EXACT && BF ? 3 : 2, PT = EXACT ? 2 : 1;
@@ -752,10 +800,10 @@ __global__ __launch_bounds__(256) void attn_dims_kernel(AttnCall c, uint32_t cls
     __shared__ uint32_t again[kRows], any_again;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t hd = c.kv.head_dim, kvh = c.kv.kv_heads;
-    const PlanHeader &head = head_of(c);
-    const AttnUnit *units = (const AttnUnit *)(c.plan + head.unit_at[cls]);
-    const uint32_t *positions = (const uint32_t *)(c.plan + head.position_at);
-    const uint32_t total = head.unit_count[cls] * kvh;
+    const UnitList list = units_of<kClass>(c);
+    const AttnUnit *units = list.units;
+    const uint32_t *positions = list.positions;
+    const uint32_t total = list.count * kvh;
 
     for (uint32_t job = blockIdx.x; job < total; job += gridDim.x) {
         const uint32_t h = job % kvh;
@@ -774,12 +822,10 @@ __global__ __launch_bounds__(256) void attn_dims_kernel(AttnCall c, uint32_t cls
             const T *kl = block_at(page) + ((b & 1) * 32 + key) * 8;
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-                const uint32_t ch = (wave * KS + ks) * 4 + g;
-                k[2 * ks] = k[2 * ks + 1] = u32x4{0, 0, 0, 0};
-                if (ch * 8 < hd) {
-                    k[2 * ks] = *(const u32x4 *)(kl + ch * 512);
-                    k[2 * ks + 1] = *(const u32x4 *)(kl + ch * 512 + 64);
-                }
+                const uint32_t ch = (wave * KS + ks) * 4 + g, at = min(ch, hd / 8 - 1) * 512;
+                const u32x4 none = {0, 0, 0, 0}, a = *(const u32x4 *)(kl + at), b = *(const u32x4 *)(kl + at + 64);
+                k[2 * ks] = ch * 8 < hd ? a : none;
+                k[2 * ks + 1] = ch * 8 < hd ? b : none;
             }
         };
         uint32_t b = u.kv0 / 32;
@@ -792,19 +838,28 @@ __global__ __launch_bounds__(256) void attn_dims_kernel(AttnCall c, uint32_t cls
         uint32_t lo[NB], hi[NB];
         {
             float v[NB][KS][8];
+            uint64_t q0[NB];
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) {
                 const uint32_t r = nb * 16 + n16;
                 const bool there = r < u.rows;
                 const RowAt at = row_at(c, u.row0 + (there ? r : 0), h);
-                const uint64_t q0 = at.token * c.q_stride + (uint64_t)at.head * hd;
+                q0[nb] = at.token * c.q_stride + (uint64_t)at.head * hd;
                 lo[nb] = 0;
                 hi[nb] = 0xffffffffu;
                 if (there) seen(c, positions[at.token], lo[nb], hi[nb]);
-#pragma unroll
-                for (int ks = 0; ks < KS; ks++)
-                    load_eight<BF>(c.q, c.q_type == kF32, q0 + min((wave * KS + ks) * 4 + g, hd / 8 - 1) * 8, v[nb][ks]);
             }
+            const auto load = [&](bool f32) {
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++)
+                        load_eight<BF>(c.q, f32, q0[nb] + min((wave * KS + ks) * 4 + g, hd / 8 - 1) * 8, v[nb][ks]);
+            };
+            if (c.q_type == kF32)
+                load(true);
+            else
+                load(false);
             if (!BF) {
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++) {
@@ -871,10 +926,7 @@ __global__ __launch_bounds__(256) void attn_dims_kernel(AttnCall c, uint32_t cls
             scores_met();
             u32x4 v[DB];
 #pragma unroll
-            for (int db = 0; db < DB; db++) {
-                const uint32_t d = (wave * DB + db) * 16 + n16;
-                v[db] = *(const u32x4 *)(vp + min(d, hd - 1) * 8);
-            }
+            for (int db = 0; db < DB; db++) v[db] = *(const u32x4 *)(vp + min((wave * DB + db) * 16 + n16, hd - 1) * 8);
             const uint32_t t0 = b * 32;
             const bool whole = t0 >= u.full0 && t0 + 32 <= u.full1;
             u32x4 p[PT][NB];
@@ -958,7 +1010,7 @@ __global__ __launch_bounds__(256) void attn_dims_kernel(AttnCall c, uint32_t cls
             }
         }
         __syncthreads();
-        if (any_again) careful_rows<BF>(c, u, h, 4, again);
+        if (any_again) careful_rows<BF>(c, u, h, 4, again, positions);
         __syncthreads();
     }
 }
@@ -975,10 +1027,10 @@ __global__ __launch_bounds__(64 * kJoinRows) void attn_join_kernel(AttnCall c) {
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t hd = c.kv.head_dim, kvh = c.kv.kv_heads;
-    const PlanHeader &head = head_of(c);
-    const JoinItem *items = (const JoinItem *)(c.plan + head.join_at);
-    const uint32_t *parts = (const uint32_t *)(c.plan + head.part_at);
-    const uint32_t total = head.join_count * kvh;
+    const PlanHeader &head = *(const PlanHeader *)c.plan;
+    const JoinItem *items = (const JoinItem *)(c.plan + (c.captured ? head.join_at : c.head.join_at));
+    const uint32_t *parts = (const uint32_t *)(c.plan + (c.captured ? head.part_at : c.head.part_at));
+    const uint32_t total = (c.captured ? head.join_count : c.head.join_count) * kvh;
     const uint32_t d = lane * V < hd ? lane * V : 0;  // lanes past the head do the first dims' work again
     for (uint32_t job = blockIdx.x; job < total; job += gridDim.x) {
         const uint32_t h = job % kvh;
@@ -1072,39 +1124,42 @@ template <bool BF, int D, bool EXACT>
 static hipError_t launch_split(hipStream_t s, uint32_t cls, uint32_t grid, const AttnCall &call) {
     if constexpr (D > 256) {
         if (cls == 0)
-            attn_dims_kernel<BF, D, 1, EXACT><<<grid, 256, 0, s>>>(call, cls);
+            attn_dims_kernel<BF, D, 1, EXACT><<<grid, 256, 0, s>>>(call);
         else
-            attn_dims_kernel<BF, D, some_blocks(D), EXACT><<<grid, 256, 0, s>>>(call, cls);
+            attn_dims_kernel<BF, D, some_blocks(D), EXACT><<<grid, 256, 0, s>>>(call);
     } else {
         if (cls == 0)
-            attn_split_kernel<BF, D, 1, EXACT><<<grid, 64 * kSplitWaves, 0, s>>>(call, cls);
+            attn_split_kernel<BF, D, 1, EXACT><<<grid, 64 * kSplitWaves, 0, s>>>(call);
         else
-            attn_split_kernel<BF, D, some_blocks(D), EXACT><<<grid, 64 * kSplitWaves, 0, s>>>(call, cls);
+            attn_split_kernel<BF, D, some_blocks(D), EXACT><<<grid, 64 * kSplitWaves, 0, s>>>(call);
     }
     return hipGetLastError();
 }
 
 template <bool BF, int D, int QT>
-static hipError_t launch_tile(hipStream_t s, uint32_t cls, uint32_t grid, const AttnCall &call) {
+static hipError_t launch_tile(hipStream_t s, uint32_t grid, const AttnCall &call) {
     constexpr uint32_t kLds = 2 * 2 * D * kPageTokens * 2;
     static LdsLimit limit;
     const hipError_t e = limit.ensure((const void *)attn_tile_kernel<BF, D, QT, tile_waves(D)>, kLds);
     if (e != hipSuccess) return e;
-    attn_tile_kernel<BF, D, QT, tile_waves(D)><<<grid, 64 * tile_waves(D), kLds, s>>>(call, cls);
+    attn_tile_kernel<BF, D, QT, tile_waves(D)><<<grid, 64 * tile_waves(D), kLds, s>>>(call);
     return hipGetLastError();
 }
 
 template <bool BF>
-static hipError_t launch_tile_dim(hipStream_t s, uint32_t cls, uint32_t grid, const AttnCall &call) {
+static hipError_t launch_tile_dim(hipStream_t s, uint32_t grid, const AttnCall &call) {
     const uint32_t hd = call.kv.head_dim;
-    if (call.q_type == kF32) {
-        if (hd <= 64) return launch_tile<BF, 64, 2>(s, cls, grid, call);
-        if (hd <= 128) return launch_tile<BF, 128, 2>(s, cls, grid, call);
-        return launch_tile<BF, 256, 2>(s, cls, grid, call);
+    // One value of a 32-bit query is enough where it is F16 and the result BF16,
+    // whose half step is eight times the query's: 4100 positions of 16 on 8 x 256,
+    // window 1024, take 157 us with two and 110 with one.
+    if (call.q_type == kF32 && (BF || call.out_type != kBF16)) {
+        if (hd <= 64) return launch_tile<BF, 64, 2>(s, grid, call);
+        if (hd <= 128) return launch_tile<BF, 128, 2>(s, grid, call);
+        return launch_tile<BF, 256, 2>(s, grid, call);
     }
-    if (hd <= 64) return launch_tile<BF, 64, 1>(s, cls, grid, call);
-    if (hd <= 128) return launch_tile<BF, 128, 1>(s, cls, grid, call);
-    return launch_tile<BF, 256, 1>(s, cls, grid, call);
+    if (hd <= 64) return launch_tile<BF, 64, 1>(s, grid, call);
+    if (hd <= 128) return launch_tile<BF, 128, 1>(s, grid, call);
+    return launch_tile<BF, 256, 1>(s, grid, call);
 }
 
 template <bool BF, bool EXACT>
@@ -1117,7 +1172,7 @@ static hipError_t launch_dim(hipStream_t s, uint32_t cls, uint32_t grid, const A
 }
 
 hipError_t launch_attn_pages(hipStream_t s, uint32_t cls, bool bf16, bool exact, uint32_t grid, const AttnCall &call) {
-    if (cls == 2) return bf16 ? launch_tile_dim<true>(s, cls, grid, call) : launch_tile_dim<false>(s, cls, grid, call);
+    if (cls == 2) return bf16 ? launch_tile_dim<true>(s, grid, call) : launch_tile_dim<false>(s, grid, call);
     if (bf16) return exact ? launch_dim<true, true>(s, cls, grid, call) : launch_dim<true, false>(s, cls, grid, call);
     return exact ? launch_dim<false, true>(s, cls, grid, call) : launch_dim<false, false>(s, cls, grid, call);
 }

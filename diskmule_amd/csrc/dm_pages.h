@@ -536,9 +536,13 @@ class Planner {
             range(*l, r, &a, &b);
             bounds(*l, r, &low, &high);
             if (a == b) continue;
-            // even chunks of whole pages, as many as come nearest to the wanted length
-            const uint64_t pages = (b - a + kPageTokens - 1) / kPageTokens;
-            const uint64_t n = plain_ ? 1 : std::max<uint64_t>(1, std::min(pages, (b - a + chunk_[l->cls] / 2) / chunk_[l->cls]));
+            // Even chunks of whole pages, as many as come nearest to the wanted
+            // length; where many rows are joined, only up to three quarters more
+            // (prompts of 1 to 2048 tokens 82 us, against 87 with the nearest;
+            // drafted tokens of 8 sequences the other way 69 against 65).
+            const uint64_t pages = (b - a + kPageTokens - 1) / kPageTokens, chunk = chunk_[l->cls];
+            const uint64_t more = l->cls == kUnitClasses - 1 ? chunk / 4 : chunk / 2;
+            const uint64_t n = plain_ ? 1 : std::max<uint64_t>(1, std::min(pages, (b - a + more) / chunk));
             const bool direct = alone && n == 1;
             const uint64_t full0 = shape_.window && high + 1ull > shape_.window ? high + 1 - shape_.window : 0;
             for (uint64_t i = 0; i < n; i++) {

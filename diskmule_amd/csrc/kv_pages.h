@@ -34,6 +34,8 @@ struct PagesView {
 struct AttnCall {
     PagesView kv;
     const uint8_t *plan;  // PlanHeader and its lists
+    PlanHeader head;      // the same head, where `captured` is not set: a load less to wait for
+    uint32_t captured;
     const void *q;
     void *out;
     uint64_t q_stride, out_stride;  // elements from one token's row to the next

@@ -668,6 +668,8 @@ int dmhip_attention_pages_device(dmhip_ctx *ctx, const dmhip_kv_plan *plan, size
     AttnCall call{};
     call.kv = pool->view((uint32_t)layer);
     call.plan = plan->lists;
+    call.head = plan->head;
+    call.captured = captured;
     call.q = query;
     call.out = output;
     call.q_stride = query_stride;
