@@ -110,18 +110,19 @@ __device__ __forceinline__ void store_one(void *p, uint32_t type, uint64_t i, fl
         ((_Float16 *)p)[i] = (_Float16)v;
 }
 
+typedef uint32_t u32x2w __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u32x2w four_halves(uint32_t type, floatx4 v) {
+    if (type == kBF16) return u32x2w{pack2<__bf16>(v[0], v[1]), pack2<__bf16>(v[2], v[3])};
+    return u32x2w{pack2<_Float16>(v[0], v[1]), pack2<_Float16>(v[2], v[3])};
+}
+
 __device__ __forceinline__ void store_four(void *p, uint32_t type, uint64_t i, floatx4 v) {
     typedef uint32_t u32x2a2 __attribute__((ext_vector_type(2), aligned(2)));
     if (type == kF32) {
         *(f32x4a4 *)((float *)p + i) = v;
         return;
     }
-    u32x2a2 w;
-    if (type == kBF16)
-        w = u32x2a2{pack2<__bf16>(v[0], v[1]), pack2<__bf16>(v[2], v[3])};
-    else
-        w = u32x2a2{pack2<_Float16>(v[0], v[1]), pack2<_Float16>(v[2], v[3])};
-    *(u32x2a2 *)((uint16_t *)p + i) = w;
+    *(u32x2a2 *)((uint16_t *)p + i) = four_halves(type, v);
 }
 
 __device__ __forceinline__ void store_two(void *p, uint32_t type, uint64_t i, float a, float b) {
@@ -142,11 +143,10 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 // of operands at a time, not all that could be asked for at once.
 __device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
 
-// 16 bytes a lane from `offset` of a buffer straight to LDS, lane l's to dst +
-// 16 l; the wave counts it like a load.
-__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t src, uint32_t offset, void *dst, uint32_t lane) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void *)dst, 16, (int)(lane * 16),
-                                             (int)offset, 0, 0);
+// 16 bytes a lane, from `offset` of a buffer, straight to LDS, lane l's to dst +
+// 16 l; zeros past the buffer's end; the wave counts it like a load.
+__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t src, uint32_t offset, void *dst) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void *)dst, 16, (int)offset, 0, 0, 0);
 }
 // What this wave has asked for with to_lds has arrived, and then what every
 // wave has; and every wave is done with what it read from LDS before.
@@ -566,15 +566,15 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
 //
 // QT: values of the page type that a query is split into (two for most 32-bit
 // queries, whose rounding would be the largest error of the result).
-template <bool BF, int D, int QT, int NW>
-__global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(AttnCall c) {
+template <bool BF, int D, int QT>
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(AttnCall c) {
     constexpr uint32_t kClass = 2;
     typedef typename Page<BF>::T T;
-    constexpr int kRows = 32 * NW, KS = D / 16, DB = D / 32;
+    constexpr int NW = 4, kRows = 32 * NW, KS = D / 16, DB = D / 32;
     constexpr int kHalf = D * kPageTokens * 2;  // bytes of a page's keys in LDS, and of its values
     constexpr float kLift = BF ? 0.0f : 10.0f, kSlack = 5.0f;
     constexpr int kSteps = 2 * KS + 4 * DB;  // products of a page, by their first operand from LDS
-    constexpr int kDeep = D <= 128 ? 4 : 6;
+    constexpr int kDeep = D <= 128 ? 4 : 6;  // reads of LDS ahead of their products
     extern __shared__ __attribute__((aligned(16))) uint8_t stage[];  // keys, keys, values, values
     __shared__ uint32_t again[kRows], any_again;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -583,9 +583,6 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
     const AttnUnit *units = list.units;
     const uint32_t *positions = list.positions;
     const uint32_t total = list.count * kvh;
-    // key dims that the pages do not hold are zero for good: no page is copied there
-    for (uint32_t i = hd * kPageTokens * 2 + threadIdx.x * 16; i < (uint32_t)kHalf; i += 64 * NW * 16)
-        *(u32x4 *)(stage + i) = *(u32x4 *)(stage + kHalf + i) = u32x4{0, 0, 0, 0};
 
     for (uint32_t job = blockIdx.x; job < total; job += gridDim.x) {
         const uint32_t h = job % kvh;
@@ -593,6 +590,9 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
         const uint32_t tid = thread_here(), lane = tid & 63u, n32 = lane & 31u, half = lane >> 5;
         if (tid < kRows) again[tid] = 0;
         if (tid == 0) any_again = 0;
+        // key dims that the pages do not hold: no page is copied there
+        for (uint32_t i = hd * kPageTokens * 2 + tid * 16; i < (uint32_t)kHalf; i += 64 * NW * 16)
+            *(u32x4 *)(stage + i) = *(u32x4 *)(stage + kHalf + i) = u32x4{0, 0, 0, 0};
         const uint32_t *table = c.kv.table + (uint64_t)u.seq * c.kv.row;
         // a page's keys (at 0) or values (at kHalf) into buffer 0 or 1 of them
         const auto fetch = [&](uint32_t page, uint32_t values, uint32_t buffer) {
@@ -604,7 +604,7 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
 #pragma unroll
             for (uint32_t k = 0; k < D / 8 / NW; k++) {
                 const uint32_t i = k * NW + wave;
-                if (i < pieces) to_lds(src, i * 1024, dst + i * 1024, lane);
+                if (i < pieces) to_lds(src, i * 1024 + lane * 16, dst + i * 1024);
             }
         };
         const uint32_t first = u.kv0 / kPageTokens, last = (u.kv1 - 1) / kPageTokens;
@@ -742,24 +742,30 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
         }
 
         l += __shfl_xor(l, 32, 64);
+        __syncthreads();  // the last page is read: its place takes the results
         // found again here rather than kept in registers all along
-        const uint32_t id = thread_here();
-        const uint32_t r1 = (id >> 6) * 32 + (id & 31), half1 = (id >> 5) & 1;
+        const uint32_t id = thread_here(), n1 = id & 31, half1 = (id >> 5) & 1, lane1 = id & 63;
+        const uint32_t r1 = wave * 32 + n1;
+        const bool direct = u.part == kNoPart;
+        constexpr uint32_t kPitch = D * 2 + 16;  // bytes of a row in LDS: rows start 4 banks apart
+        uint8_t *mine = stage + wave * (32 * kPitch + 256);
+        uint64_t *row_to = (uint64_t *)(mine + 32 * kPitch);
         if (r1 < u.rows) {
-            const RowAt to = row_at(c, u.row0 + r1, h);
             bool odd = false;
 #pragma unroll
             for (int db = 0; db < DB; db++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) odd |= db * 32 + 8 * (i >> 2) < (int)hd && !finite(acc[db][i]);
             if (odd || !finite(l)) again[r1] = any_again = 1;
-            const bool direct = u.part == kNoPart;
             const uint64_t slot = (uint64_t)(u.part + r1) * kvh + h;
             if (half1 == 0) {
-                if (!direct)
+                if (!direct) {
                     c.part_ml[slot] = float2{m - kLift, l};
-                else if (l == 0.0f)
-                    *c.bad.word = c.bad.mark;
+                } else {
+                    const RowAt to = row_at(c, u.row0 + r1, h);
+                    row_to[n1] = to.token * c.out_stride + (uint64_t)to.head * hd;
+                    if (l == 0.0f) *c.bad.word = c.bad.mark;
+                }
             }
             const float over = 1.0f / l;
 #pragma unroll
@@ -767,13 +773,23 @@ __global__ __launch_bounds__(64 * NW, D <= 128 ? 2 : 1) void attn_tile_kernel(At
 #pragma unroll
                 for (int a = 0; a < 4; a++) {
                     const uint32_t d = db * 32 + a * 8 + half1 * 4;
-                    if (d >= hd) continue;
                     const floatx4 o = {acc[db][a * 4], acc[db][a * 4 + 1], acc[db][a * 4 + 2], acc[db][a * 4 + 3]};
                     if (direct)
-                        store_four(c.out, c.out_type, to.token * c.out_stride + (uint64_t)to.head * hd + d, o * over);
-                    else
+                        *(u32x2w *)(mine + n1 * kPitch + d * 2) = four_halves(c.out_type, o * over);
+                    else if (d < hd)
                         *(f32x4a4 *)(c.part_o + slot * hd + d) = o;
                 }
+        }
+        if (direct) {
+            // rows go out whole, 16 bytes a lane; the wave's own LDS, so no barrier
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            constexpr uint32_t kLanes = D / 8;  // of a row
+#pragma unroll
+            for (uint32_t r0 = 0; r0 < 32; r0 += 64 / kLanes) {
+                const uint32_t r = r0 + lane1 / kLanes, d = lane1 % kLanes * 8;
+                if (wave * 32 + r < u.rows && d < hd)
+                    *(u32x4a2 *)((uint16_t *)c.out + row_to[r] + d) = *(const u32x4 *)(mine + r * kPitch + d * 2);
+            }
         }
         __syncthreads();
         if (any_again) careful_rows<BF>(c, u, h, NW, again, positions);
@@ -1105,11 +1121,9 @@ __global__ __launch_bounds__(64 * kJoinRows) void attn_join_kernel(AttnCall c) {
 
 static constexpr int some_blocks(int d) { return d <= 128 ? 4 : d <= 256 ? 2 : 3; }
 
-static constexpr int tile_waves(int d) { return 4; }
-
 uint32_t attn_pages_rows(uint32_t cls, uint32_t head_dim, bool exact) {
     if (cls == 0) return 16;
-    if (cls == 2) return exact || head_dim > 256 ? 0 : 32 * tile_waves(head_dim <= 128 ? 128 : 256);
+    if (cls == 2) return exact || head_dim > 256 ? 0 : 128;
     return 16 * some_blocks(head_dim <= 128 ? 128 : head_dim <= 256 ? 256 : 512);
 }
 
@@ -1140,9 +1154,9 @@ template <bool BF, int D, int QT>
 static hipError_t launch_tile(hipStream_t s, uint32_t grid, const AttnCall &call) {
     constexpr uint32_t kLds = 2 * 2 * D * kPageTokens * 2;
     static LdsLimit limit;
-    const hipError_t e = limit.ensure((const void *)attn_tile_kernel<BF, D, QT, tile_waves(D)>, kLds);
+    const hipError_t e = limit.ensure((const void *)attn_tile_kernel<BF, D, QT>, kLds);
     if (e != hipSuccess) return e;
-    attn_tile_kernel<BF, D, QT, tile_waves(D)><<<grid, 64 * tile_waves(D), kLds, s>>>(call);
+    attn_tile_kernel<BF, D, QT><<<grid, 256, kLds, s>>>(call);
     return hipGetLastError();
 }
 
