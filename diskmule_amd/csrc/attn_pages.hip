@@ -171,6 +171,12 @@ __device__ __forceinline__ uint32_t thread_here() {
     return id;
 }
 
+// Every wave's stores are done: what is stored now comes after them.
+__device__ __forceinline__ void stores_done() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
 // A word that is the same for the whole wave, by the scalar path.
 __device__ __forceinline__ uint32_t word_at(const uint32_t *p, uint32_t i) {
     return ((const __attribute__((address_space(4))) uint32_t *)p)[i];
@@ -300,7 +306,7 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
     constexpr uint32_t kClass = NB == 1 ? 0 : 1;
     typedef typename Page<BF>::T T;
     constexpr int kRows = 16 * NB, KS = D / 32, DB = D / 16;
-    constexpr int QT = EXACT && BF ? 3 : 2, PT = EXACT ? 2 : 1;
+    constexpr int QT = EXACT && BF ? 3 : 2, PT = EXACT ? QT : 1;
     // Probabilities of F16 pages are 2^10 times larger: its smallest value 2^-24
     // would lose the many small ones of a long row.
     constexpr float kLift = BF ? 0.0f : 10.0f;
@@ -552,7 +558,10 @@ __global__ __launch_bounds__(64 * kSplitWaves) void attn_split_kernel(AttnCall c
             }
         }
         __syncthreads();
-        if (any_again) careful_rows<BF>(c, u, h, kSplitWaves, again, positions);
+        if (any_again) {
+            stores_done();
+            careful_rows<BF>(c, u, h, kSplitWaves, again, positions);
+        }
         __syncthreads();
     }
 }
@@ -792,31 +801,33 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(AttnCa
             }
         }
         __syncthreads();
-        if (any_again) careful_rows<BF>(c, u, h, NW, again, positions);
+        if (any_again) {
+            stores_done();
+            careful_rows<BF>(c, u, h, NW, again, positions);
+        }
         __syncthreads();
     }
 }
 
 // Units of heads of more than 256 dims. The waves share the dims: each has a
 // quarter of every key's and value's, so that its queries and results fit its
-// registers, and every key and value goes into one wave's registers once for up
-// to 48 rows (64 do not fit). What the waves have of a block of 32 scores meets in LDS, where
-// each reads all four and adds them in one order: m, sum and probabilities are
-// the same in every wave. Two places in turn, so that one barrier a block is
-// enough. Keys of the next block are asked for before the barrier.
-template <bool BF, int D, int NB, bool EXACT>
+// registers, and every key and value goes into one wave's registers once. What the
+// waves have of a block of 32 scores meets in LDS, where each reads all four and
+// adds them in one order: m, sum and probabilities are the same in every wave. Two
+// places in turn, so that one barrier a block is enough. Keys of the next block
+// are asked for before the barrier.
+template <bool BF, int D, bool EXACT>
 __global__ __launch_bounds__(256) void attn_dims_kernel(AttnCall c) {
-    constexpr uint32_t kClass = NB == 1 ? 0 : 1;
     typedef typename Page<BF>::T T;
-    constexpr int kRows = 16 * NB, DW = D / 4, KS = DW / 32, DB = DW / 16;
-    constexpr int QT = EXACT && BF ? 3 : 2, PT = EXACT ? 2 : 1;
+    constexpr int kRows = 16, DW = D / 4, KS = DW / 32, DB = DW / 16;
+    constexpr int QT = EXACT && BF ? 3 : 2, PT = EXACT ? QT : 1;
     constexpr float kLift = BF ? 0.0f : 10.0f, kSlack = 5.0f;
-    __shared__ floatx4 scores[2][4][2 * NB][64];
+    __shared__ floatx4 scores[2][4][2][64];
     __shared__ float row_top[4][kRows];
     __shared__ uint32_t again[kRows], any_again;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t hd = c.kv.head_dim, kvh = c.kv.kv_heads;
-    const UnitList list = units_of<kClass>(c);
+    const UnitList list = units_of<0>(c);
     const AttnUnit *units = list.units;
     const uint32_t *positions = list.positions;
     const uint32_t total = list.count * kvh;
@@ -849,160 +860,129 @@ __global__ __launch_bounds__(256) void attn_dims_kernel(AttnCall c) {
         u32x4 k[2 * KS];
         load_keys(k, page, b);
         // ---- queries: the wave's dims of every row ----
-        u32x4 q[QT][NB][KS];
-        float scale[NB];
-        uint32_t lo[NB], hi[NB];
+        u32x4 q[QT][KS];
+        float scale;
+        uint32_t lo = 0, hi = 0xffffffffu;
         {
-            float v[NB][KS][8];
-            uint64_t q0[NB];
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++) {
-                const uint32_t r = nb * 16 + n16;
-                const bool there = r < u.rows;
-                const RowAt at = row_at(c, u.row0 + (there ? r : 0), h);
-                q0[nb] = at.token * c.q_stride + (uint64_t)at.head * hd;
-                lo[nb] = 0;
-                hi[nb] = 0xffffffffu;
-                if (there) seen(c, positions[at.token], lo[nb], hi[nb]);
-            }
+            float v[KS][8];
+            const uint32_t r = n16;
+            const bool there = r < u.rows;
+            const RowAt at = row_at(c, u.row0 + (there ? r : 0), h);
+            const uint64_t q0 = at.token * c.q_stride + (uint64_t)at.head * hd;
+            if (there) seen(c, positions[at.token], lo, hi);
             const auto load = [&](bool f32) {
 #pragma unroll
-                for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                    for (int ks = 0; ks < KS; ks++)
-                        load_eight<BF>(c.q, f32, q0[nb] + min((wave * KS + ks) * 4 + g, hd / 8 - 1) * 8, v[nb][ks]);
+                for (int ks = 0; ks < KS; ks++)
+                    load_eight<BF>(c.q, f32, q0 + min((wave * KS + ks) * 4 + g, hd / 8 - 1) * 8, v[ks]);
             };
             if (c.q_type == kF32)
                 load(true);
             else
                 load(false);
             if (!BF) {
+                float top = 0.0f;
 #pragma unroll
-                for (int nb = 0; nb < NB; nb++) {
-                    float top = 0.0f;
+                for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-                    for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                        for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[nb][ks][i]));
-                    top = fmaxf(top, __shfl_xor(top, 16, 64));
-                    top = fmaxf(top, __shfl_xor(top, 32, 64));
-                    if (g == 0) row_top[wave][nb * 16 + n16] = top;
-                }
+                    for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[ks][i]));
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                if (g == 0) row_top[wave][n16] = top;
                 __syncthreads();
             }
+            int e = 0;
+            if (!BF && c.q_type == kF32)
+                e = row_power(fmaxf(fmaxf(row_top[0][r], row_top[1][r]), fmaxf(row_top[2][r], row_top[3][r])));
+            scale = ldexpf(c.scale, e);
 #pragma unroll
-            for (int nb = 0; nb < NB; nb++) {
-                const uint32_t r = nb * 16 + n16;
-                int e = 0;
-                if (!BF && c.q_type == kF32)
-                    e = row_power(fmaxf(fmaxf(row_top[0][r], row_top[1][r]), fmaxf(row_top[2][r], row_top[3][r])));
-                scale[nb] = ldexpf(c.scale, e);
+            for (int ks = 0; ks < KS; ks++) {
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        v[nb][ks][i] = r < u.rows && ((wave * KS + ks) * 4 + g) * 8 < hd ? v[nb][ks][i] : 0.0f;
-                        if (!BF) v[nb][ks][i] = ldexpf(v[nb][ks][i], -e);
-                    }
-#pragma unroll
-                    for (int term = 0; term < QT; term++) q[term][nb][ks] = split8<T>(v[nb][ks]);
+                for (int i = 0; i < 8; i++) {
+                    v[ks][i] = r < u.rows && ((wave * KS + ks) * 4 + g) * 8 < hd ? v[ks][i] : 0.0f;
+                    if (!BF) v[ks][i] = ldexpf(v[ks][i], -e);
                 }
+#pragma unroll
+                for (int term = 0; term < QT; term++) q[term][ks] = split8<T>(v[ks]);
             }
         }
-        floatx4 acc[DB][NB];
+        floatx4 acc[DB];
 #pragma unroll
-        for (int db = 0; db < DB; db++)
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++) acc[db][nb] = floatx4{0, 0, 0, 0};
-        float m[NB], l[NB];
-#pragma unroll
-        for (int nb = 0; nb < NB; nb++) m[nb] = -INFINITY, l[nb] = 0.0f;
+        for (int db = 0; db < DB; db++) acc[db] = floatx4{0, 0, 0, 0};
+        float m = -INFINITY, l = 0.0f;
 
 #pragma unroll 1
         for (; b < blocks; b++) {
             const T *vp = block_at(page) + hd * kPageTokens + ((b & 1) * 4 + g) * hd * 8;
-            floatx4 s[2][NB];
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++) s[0][nb] = s[1][nb] = floatx4{0, 0, 0, 0};
+            floatx4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-                for (int term = 0; term < QT; term++)
-#pragma unroll
-                    for (int nb = 0; nb < NB; nb++) {
-                        s[0][nb] = Page<BF>::mfma(k[2 * ks], q[term][nb][ks], s[0][nb]);
-                        s[1][nb] = Page<BF>::mfma(k[2 * ks + 1], q[term][nb][ks], s[1][nb]);
-                    }
+                for (int term = 0; term < QT; term++) {
+                    s[0] = Page<BF>::mfma(k[2 * ks], q[term][ks], s[0]);
+                    s[1] = Page<BF>::mfma(k[2 * ks + 1], q[term][ks], s[1]);
+                }
             if (b + 1 < blocks) load_keys(k, page1, b + 1);
             page = page1;
             page1 = word_at(table, min(b + 2, blocks - 1) >> 1);
             floatx4(*put)[64] = scores[b & 1][wave];
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++) put[nb][lane] = s[0][nb], put[NB + nb][lane] = s[1][nb];
+            put[0][lane] = s[0], put[1][lane] = s[1];
             scores_met();
             u32x4 v[DB];
 #pragma unroll
             for (int db = 0; db < DB; db++) v[db] = *(const u32x4 *)(vp + min((wave * DB + db) * 16 + n16, hd - 1) * 8);
             const uint32_t t0 = b * 32;
             const bool whole = t0 >= u.full0 && t0 + 32 <= u.full1;
-            u32x4 p[PT][NB];
+            u32x4 p[PT];
+            in_order();
+            float x[8];
 #pragma unroll
-            for (int nb = 0; nb < NB; nb++) {
-                in_order();
-                float x[8];
+            for (int a = 0; a < 2; a++) {
+                floatx4 sum = scores[b & 1][0][a][lane];
 #pragma unroll
-                for (int a = 0; a < 2; a++) {
-                    floatx4 sum = scores[b & 1][0][a * NB + nb][lane];
+                for (int w = 1; w < 4; w++) sum += scores[b & 1][w][a][lane];
 #pragma unroll
-                    for (int w = 1; w < 4; w++) sum += scores[b & 1][w][a * NB + nb][lane];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) x[a * 4 + i] = sum[i] * scale[nb];
-                }
-                if (!whole) {
-                    const uint32_t first = t0 + 16 * (g >> 1) + 4 * (g & 1);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const uint32_t t = first + (i & 3) + 8 * (i >> 2);
-                        x[i] = t >= lo[nb] && t < hi[nb] ? x[i] : -INFINITY;
-                    }
-                }
-                float top = x[0];
-#pragma unroll
-                for (int i = 1; i < 8; i++) top = fmaxf(top, x[i]);
-                if (__any(top > m[nb] + kSlack)) {
-                    top = fmaxf(top, __shfl_xor(top, 16, 64));
-                    top = fmaxf(top, __shfl_xor(top, 32, 64));
-                    const float next = fmaxf(m[nb], top);
-                    const float keep = m[nb] == next ? 1.0f : exp2_hw(m[nb] - next);
-                    m[nb] = next;
-                    l[nb] *= keep;
-#pragma unroll
-                    for (int db = 0; db < DB; db++) acc[db][nb] = acc[db][nb] * keep;
-                }
-                const float from = (m[nb] == -INFINITY ? 0.0f : m[nb]) - kLift;
+                for (int i = 0; i < 4; i++) x[a * 4 + i] = sum[i] * scale;
+            }
+            if (!whole) {
+                const uint32_t first = t0 + 16 * (g >> 1) + 4 * (g & 1);
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    x[i] = exp2_hw(x[i] - from);
-                    l[nb] += x[i];
+                    const uint32_t t = first + (i & 3) + 8 * (i >> 2);
+                    x[i] = t >= lo && t < hi ? x[i] : -INFINITY;
                 }
-#pragma unroll
-                for (int term = 0; term < PT; term++) p[term][nb] = split8<T>(x);
             }
+            float top = x[0];
+#pragma unroll
+            for (int i = 1; i < 8; i++) top = fmaxf(top, x[i]);
+            if (__any(top > m + kSlack)) {
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float next = fmaxf(m, top);
+                const float keep = m == next ? 1.0f : exp2_hw(m - next);
+                m = next;
+                l *= keep;
+#pragma unroll
+                for (int db = 0; db < DB; db++) acc[db] = acc[db] * keep;
+            }
+            const float from = (m == -INFINITY ? 0.0f : m) - kLift;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                x[i] = exp2_hw(x[i] - from);
+                l += x[i];
+            }
+#pragma unroll
+            for (int term = 0; term < PT; term++) p[term] = split8<T>(x);
 #pragma unroll
             for (int db = 0; db < DB; db++)
 #pragma unroll
-                for (int term = 0; term < PT; term++)
-#pragma unroll
-                    for (int nb = 0; nb < NB; nb++) acc[db][nb] = Page<BF>::mfma(v[db], p[term][nb], acc[db][nb]);
+                for (int term = 0; term < PT; term++) acc[db] = Page<BF>::mfma(v[db], p[term], acc[db]);
         }
 
         const uint32_t lane1 = thread_here() & 63u, g1 = lane1 >> 4;  // as in attn_tile_kernel
-#pragma unroll
-        for (int nb = 0; nb < NB; nb++) {
-            const uint32_t r = nb * 16 + (lane1 & 15);
-            float sum = l[nb] + __shfl_xor(l[nb], 16, 64);
-            sum += __shfl_xor(sum, 32, 64);
-            if (r >= u.rows) continue;
+        const uint32_t r = lane1 & 15;
+        float sum = l + __shfl_xor(l, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (r < u.rows) {
             const RowAt at = row_at(c, u.row0 + r, h);
             const uint64_t slot = (uint64_t)(u.part + r) * kvh + h;
             bool odd = false;
@@ -1010,7 +990,7 @@ __global__ __launch_bounds__(256) void attn_dims_kernel(AttnCall c) {
             for (int db = 0; db < DB; db++) {
                 const uint32_t d = (wave * DB + db) * 16 + g1 * 4;
                 if (d >= hd) continue;
-                const floatx4 o = acc[db][nb];
+                const floatx4 o = acc[db];
                 odd |= !finite(o[0]) || !finite(o[1]) || !finite(o[2]) || !finite(o[3]);
                 if (u.part == kNoPart)
                     store_four(c.out, c.out_type, at.token * c.out_stride + (uint64_t)at.head * hd + d, o / sum);
@@ -1020,13 +1000,16 @@ __global__ __launch_bounds__(256) void attn_dims_kernel(AttnCall c) {
             if (odd || !finite(sum)) again[r] = any_again = 1;
             if (wave == 0 && g1 == 0) {
                 if (u.part != kNoPart)
-                    c.part_ml[slot] = float2{m[nb] - kLift, sum};
+                    c.part_ml[slot] = float2{m - kLift, sum};
                 else if (sum == 0.0f)
                     *c.bad.word = c.bad.mark;
             }
         }
         __syncthreads();
-        if (any_again) careful_rows<BF>(c, u, h, 4, again, positions);
+        if (any_again) {
+            stores_done();
+            careful_rows<BF>(c, u, h, 4, again, positions);
+        }
         __syncthreads();
     }
 }
@@ -1119,17 +1102,17 @@ __global__ __launch_bounds__(64 * kJoinRows) void attn_join_kernel(AttnCall c) {
     }
 }
 
-static constexpr int some_blocks(int d) { return d <= 128 ? 4 : d <= 256 ? 2 : 3; }
+static constexpr int some_blocks(int d) { return d <= 128 ? 4 : 2; }
 
 uint32_t attn_pages_rows(uint32_t cls, uint32_t head_dim, bool exact) {
     if (cls == 0) return 16;
     if (cls == 2) return exact || head_dim > 256 ? 0 : 128;
-    return 16 * some_blocks(head_dim <= 128 ? 128 : head_dim <= 256 ? 256 : 512);
+    return head_dim <= 256 ? 16 * some_blocks(head_dim <= 128 ? 128 : 256) : 0;
 }
 
 // By their registers and LDS, which the build reports.
 uint32_t attn_pages_resident(uint32_t cls, uint32_t head_dim) {
-    if (cls == 0) return 2;
+    if (cls == 0) return head_dim > 128 && head_dim <= 256 ? 1 : 2;
     if (cls == 1) return head_dim <= 64 ? 2 : 1;
     return head_dim <= 128 ? 2 : 1;
 }
@@ -1137,10 +1120,7 @@ uint32_t attn_pages_resident(uint32_t cls, uint32_t head_dim) {
 template <bool BF, int D, bool EXACT>
 static hipError_t launch_split(hipStream_t s, uint32_t cls, uint32_t grid, const AttnCall &call) {
     if constexpr (D > 256) {
-        if (cls == 0)
-            attn_dims_kernel<BF, D, 1, EXACT><<<grid, 256, 0, s>>>(call);
-        else
-            attn_dims_kernel<BF, D, some_blocks(D), EXACT><<<grid, 256, 0, s>>>(call);
+        attn_dims_kernel<BF, D, EXACT><<<grid, 256, 0, s>>>(call);
     } else {
         if (cls == 0)
             attn_split_kernel<BF, D, 1, EXACT><<<grid, 64 * kSplitWaves, 0, s>>>(call);
@@ -1165,7 +1145,7 @@ static hipError_t launch_tile_dim(hipStream_t s, uint32_t grid, const AttnCall &
     const uint32_t hd = call.kv.head_dim;
     // One value of a 32-bit query is enough where it is F16 and the result BF16,
     // whose half step is eight times the query's: 4100 positions of 16 on 8 x 256,
-    // window 1024, take 157 us with two and 110 with one.
+    // window 1024, take 157 us with two and 138 with one.
     if (call.q_type == kF32 && (BF || call.out_type != kBF16)) {
         if (hd <= 64) return launch_tile<BF, 64, 2>(s, grid, call);
         if (hd <= 128) return launch_tile<BF, 128, 2>(s, grid, call);

@@ -332,6 +332,7 @@ struct PlanShape {
     uint32_t rows_of[kUnitClasses] = {16, 64, 0};
     uint32_t workgroups[kUnitClasses] = {512, 512, 512};  // wanted of a launch
     uint32_t least_chunk[kUnitClasses] = {256, 256, 512}; // positions of a unit, at least, where it is split
+    uint32_t short_positions = 0, short_rounds = 0;       // of units that the smallest kernel takes whatever the rows
     uint32_t share_pages = 2;                             // whole pages in common from which rows share a unit
     size_t max_parts = 0;                                 // partial rows (per KV head)
     size_t max_bytes = 0;                                 // of the lists
@@ -418,9 +419,18 @@ class Planner {
         paths_.clear();
         std::vector<size_t> path;
         split(0, items_.size(), 0, path);
-        // one launch for all: of the kernel that the most rows need
+        // One launch for all: of the kernel that the most rows need, or of the
+        // one for few rows where its units are short and at work in few rounds:
+        // 16 rows go through their positions sooner than 64 or 128 do, and read
+        // those again from the caches.
         uint32_t cls = 0;
-        for (const Level &l : levels_) cls = std::max(cls, class_of(l.rows));
+        uint64_t longest = 0, small = 0;
+        for (const Level &l : levels_) {
+            cls = std::max(cls, class_of(l.rows));
+            longest = std::max(longest, l.kv1 - l.kv0);
+            small += (l.rows + shape_.rows_of[0] - 1) / shape_.rows_of[0];
+        }
+        if (longest <= shape_.short_positions && small * shape_.kv_heads <= shape_.short_rounds * shape_.workgroups[0]) cls = 0;
         for (Level &l : levels_) {
             l.cls = cls;
             l.tile = shape_.rows_of[cls];

@@ -543,6 +543,13 @@ int dmhip_new_kv_plan(dmhip_kv_pages *pool, size_t query_heads, int has_window, 
         s.workgroups[c] = attn_pages_resident(c, pool->head_dim) * cus;
         most = std::max(most, s.rows_of[c]);
     }
+    // Short prompts, the whole call in us with the kernel for few rows and with
+    // the one that their rows ask for: 32 heads on 8 x 128, F32 results of 256
+    // positions 9 and 17, 700 29 and 33, 1024 equal; 16-bit results of 400 14 and
+    // 15, 512 16 and 16, 700 24 and 20; 16 on 8 x 256, 256 positions 11 and 17,
+    // 512 33 and 32.
+    s.short_positions = 1024;
+    s.short_rounds = pool->head_dim > 128 ? 1 : output_type == kF32 ? 4 : 2;
     const size_t sequences = std::min<size_t>(pool->book.sequences(), max_tokens);
     s.max_parts = 2 * std::min(rows, sequences * kSharedRows) + 4 * (size_t)cus * most / pool->kv_heads + most;
     s.max_bytes = plan_least_bytes(max_tokens, group, sequences) + std::min(rows, s.max_parts / 2) * sizeof(JoinItem) + (512u << 10);

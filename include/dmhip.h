@@ -597,14 +597,17 @@ int dmhip_kv_pages_compact(dmhip_kv_pages *pool, size_t *moved);
    work on them is laid out over the device.  query_heads is a multiple of the
    cache's kv_heads; with has_window a token sees the last sliding_window
    tokens up to itself, else all.  query_type: F32 or the cache's type;
-   output_type: F32, F16 or BF16.  With 16-bit output, queries and
-   probabilities are rounded to the cache's type once; with F32 output both
-   are split into two or three such values, which leaves an error of about
-   2^-17 of a probability.  All sums are 32-bit.  Holds device memory for
-   max_tokens tokens a step (and nothing grows later). */
+   output_type: F32, F16 or BF16.  Products are of the cache's type: a 32-bit
+   query is split into two such values (three for BF16 with F32 output; one,
+   rounded, for F16 pages with BF16 output), a probability is rounded once for
+   16-bit output and split for F32 output into three values (BF16) or two (F16),
+   which leaves an error of 2^-24 or 2^-22 of it.  Sums, and the softmax's
+   statistics, are 32-bit.  Holds device memory for max_tokens tokens a step
+   (and nothing grows later). */
 int dmhip_new_kv_plan(dmhip_kv_pages *pool, size_t query_heads, int has_window, size_t sliding_window,
                       uint32_t query_type, uint32_t output_type, size_t max_tokens, dmhip_kv_plan **out);
-/* Waits for the context's stream first. */
+/* Waits for the context's stream first.  Graphs that hold calls of the plan, or
+   of its cache, must not be replayed once either is freed. */
 void dmhip_kv_plan_free(dmhip_kv_plan *plan);
 /* The step's tokens: the last tokens[i] tokens of each of `count` distinct
    sequences, packed in this order wherever the calls below take or give rows.

@@ -7,11 +7,13 @@ Tolerances.  With u = 2^-24 (32-bit sums), h(T) half a step of a 16-bit type
 (bf16 2^-9 of the value's binade at most 2^-8 relative: finfo.eps / 2), S the
 largest sum |q_d k_d| * scale of a row, n its positions, A = sum_j p_j |v_j|:
   * a score is off by at most (head_dim + 4) u S from the 32-bit sum, and by
-    h(page type) S more where a 32-bit query is rounded to the page type;
-    2^-22 S where it is split into two or three values of it;
+    what is left of a 32-bit query: h(page type) S where it is rounded to the
+    page type (F16 pages, BF16 results), its square where it is split in two,
+    2^-22 S for 32-bit results (BF16 in three, F16 in two);
   * a probability is off by that, by 2 u of its exponential, relatively; the
     sum of them by as much, so the quotient by twice that;
-  * rounding it to the page type adds h(T), or h(T)^2 where it is split in two;
+  * rounding it to the page type adds h(T); for 32-bit results h(T)^2 (F16, split
+    in two) or h(T)^3 (BF16, in three);
   * F16 probabilities, 2^10 times larger, vanish below 2^-35: n 2^-35;
   * sums of n terms add n u; the result's own rounding h(output) |o|.
 """
@@ -202,9 +204,10 @@ class Model:
         o, spread, size, n = self.expect(seqs, counts, q, window, scale, layer)
         n = n[:, None, None]
         exact = out_type == F32
-        query = 2.0 ** -22 if exact else (HALF[self.kind] if q_type == F32 else 0.0)
+        once = self.kind == F16 and out_type == BF16
+        query = 2.0 ** -22 if exact else 0.0 if q_type != F32 else HALF[self.kind] if once else HALF[self.kind] ** 2
         score = ((self.hd + 4) * U + query) * spread[:, :, None]
-        p = HALF[self.kind] ** 2 if exact else HALF[self.kind]
+        p = HALF[self.kind] ** ((3 if self.kind == BF16 else 2) if exact else 1)
         bound = (2 * (score + 2 * U) + p + (n + 8) * U) * size * 1.01 + n * 2.0 ** -35 * np.abs(o).max() + \
             HALF[out_type] * np.abs(o) * 1.01 + 1e-30
         worst = np.abs(got - o) / bound
@@ -335,9 +338,10 @@ def test_prompts_of_different_lengths(ctx, heads, kvh, hd, kind, q_type, out_typ
 
 @pytest.mark.parametrize("window", [1, 2, 31, 64, 65, 1000])
 @pytest.mark.parametrize("kind,out_type", [(BF16, F32), (F16, F16)])
-def test_windows(ctx, window, kind, out_type):
+@pytest.mark.parametrize("hd", [64, 256, 512])
+def test_windows(ctx, window, kind, out_type, hd):
     rng = np.random.default_rng(window)
-    m = Model(ctx, kind, 2, 64)
+    m = Model(ctx, kind, 2, hd)
     seqs = [m.new() for _ in range(4)]
     m.grow(seqs, [300, 1, 200, 64], rng)
     m.attend(seqs, [300, 1, 90, 2], rng, 6, window=window, out_type=out_type)
@@ -441,7 +445,7 @@ def test_a_row_of_many_small_probabilities(ctx):
 
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("kind,out_type", [(BF16, F32), (BF16, BF16), (F16, F32), (F16, F16)])
-@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("hd", [24, 64, 72, 128, 136, 256, 264, 512])
 def test_unseen_places_reach_no_result(ctx, bad, kind, out_type, hd):
     rng = np.random.default_rng(13)
     m = Model(ctx, kind, 1, hd, pages=30, sequences=6)

@@ -46,12 +46,15 @@ size_t work_tables(Book *b, uint32_t *out) {
     if (out) memcpy(out, b->work.tables.data(), b->work.tables.size() * 12);
     return b->work.tables.size();
 }
+uint32_t short_of[2] = {0, 0};
+void shorts(uint32_t positions, uint32_t rounds) { short_of[0] = positions; short_of[1] = rounds; }
 void plan(Book *b, uint32_t group, uint32_t kv_heads, uint64_t window, const uint32_t *rows, const uint32_t *wgs,
           const uint32_t *least, uint32_t share, size_t max_parts, size_t max_bytes, size_t n, const size_t *s,
           const size_t *c) {
     PlanShape p;
     p.group = group; p.kv_heads = kv_heads; p.window = window; p.share_pages = share;
     for (int i = 0; i < 3; i++) p.rows_of[i] = rows[i], p.workgroups[i] = wgs[i], p.least_chunk[i] = least[i];
+    p.short_positions = short_of[0]; p.short_rounds = short_of[1];
     p.max_parts = max_parts; p.max_bytes = max_bytes;
     Planner(b->book, p, n, s, c).build(&b->lists);
 }
@@ -88,7 +91,7 @@ def lib(tmp_path_factory):
                        "book_refs": [vp, u32], "book_length": [vp, sz], "book_version": [vp, sz],
                        "book_writable": [vp, sz, u64], "book_table": [vp, sz, vp], "work_copies": [vp, vp],
                        "work_tables": [vp, vp], "lists_bytes": [vp], "lists_part_rows": [vp],
-                       "plan_least": [sz, sz, sz], "list": [vp, ctypes.c_int, vp],
+                       "plan_least": [sz, sz, sz], "shorts": [u32, u32], "list": [vp, ctypes.c_int, vp],
                        "plan": [vp, u32, u32, u64, vp, vp, vp, u32, sz, sz, sz, vp, vp]}.items():
         getattr(lib, name).argtypes = args
     for name in ("book_table", "work_copies", "work_tables", "lists_bytes", "lists_part_rows", "plan_least", "list"):
@@ -408,4 +411,26 @@ def test_a_shared_prefix_is_one_unit_for_all(lib):
     assert len(shared) == 1 and shared[0][3] == 0 and shared[0][4] == 15 * PAGE
     # each sequence's own: the partly filled page and its token
     assert sorted(tuple(u[3:5]) for u in units if u[1] != 32) == [(15 * PAGE, 1001)] * 8
+    c.close()
+
+
+@pytest.mark.parametrize("tokens,group,short,cls", [
+    (300, 2, (512, 4), 0),    # 38 units of 16 rows, 64 at once
+    (300, 2, (512, 2), 2),    # 32 at once
+    (300, 2, (256, 4), 2),    # too long
+    (512, 2, (512, 4), 0),    # 64 units exactly
+    (513, 2, (1024, 4), 2),
+    (300, 2, (0, 0), 2),
+])
+def test_short_units_that_are_at_work_at_once_go_to_the_smallest_kernel(lib, tokens, group, short, cls):
+    c = Cache(lib, 200, 4, 4096)
+    c.create()
+    c.extend([0], [tokens])
+    lib.shorts(*short)
+    try:
+        for room in (10 ** 9, 0):  # of the lists: the least has to do
+            check_plan(lib, c, [0], [tokens], group, 2, 0, [16, 64, 128], [32] * 3, [256] * 3, 2, 10 ** 9, room)
+            assert [bool(len(lists(lib, c.b, k, 8))) for k in range(3)] == [k == cls for k in range(3)]
+    finally:
+        lib.shorts(0, 0)
     c.close()
