@@ -363,6 +363,7 @@ constexpr size_t plan_least_bytes(size_t tokens, size_t group, size_t sequences)
 
 class Planner {
    public:
+    static constexpr size_t kDeepest = 32;  // levels above a sequence's own
     Planner(const PageBook &book, const PlanShape &shape, size_t n, const size_t *seqs, const size_t *counts)
         : book_(book), shape_(shape) {
         uint32_t token = 0;
@@ -464,12 +465,13 @@ class Planner {
 
     // Sequences lo .. hi - 1 hold their first `from` pages in common, and those
     // are dealt with (levels of `path`): units for what follows.  A run of
-    // sequences that begin alike is found by its neighbours' common pages.
+    // sequences that begin alike is found by its neighbours' common pages.  Only
+    // so deep: a row has a part of each level, and every sequence its path.
     void split(size_t lo, size_t hi, uint32_t from, std::vector<size_t> &path) {
         while (lo < hi) {
             size_t end = lo + 1;
             uint32_t common = UINT32_MAX;
-            while (!plain_ && end < hi && common_[end - 1] >= from + shape_.share_pages) {
+            while (!plain_ && path.size() < kDeepest && end < hi && common_[end - 1] >= from + shape_.share_pages) {
                 common = std::min(common, common_[end - 1]);
                 end++;
             }

@@ -556,6 +556,10 @@ int dmhip_new_kv_plan(dmhip_kv_pages *pool, size_t query_heads, int has_window, 
     s.max_parts = 2 * std::min(rows, sequences * kSharedRows) + 4 * (size_t)cus * most / pool->kv_heads + most;
     s.max_bytes = plan_least_bytes(max_tokens, group, sequences) + std::min(rows, s.max_parts / 2) * sizeof(JoinItem) + (512u << 10);
     p->list_bytes = sizeof(PlanHeader) + s.max_bytes + 16 * 8;
+    if (p->list_bytes > 0xffffffffu) {  // places in the lists are 32-bit
+        plan_release(p);
+        return fail(DMHIP_ERR_VECTOR_TOO_LARGE, "HIP vector length exceeds the 32-bit kernel limit");
+    }
     const size_t part_rows = s.max_parts * pool->kv_heads;
     const size_t sizes[3] = {p->list_bytes, part_rows * pool->head_dim * 4, part_rows * sizeof(float2)};
     void **places[3] = {(void **)&p->lists, (void **)&p->part_o, (void **)&p->part_ml};
@@ -614,6 +618,7 @@ int dmhip_kv_plan_set(dmhip_kv_plan *plan, size_t count, const size_t *sequences
     const int slot = plan->next;
     DM_HIP(hipEventSynchronize(plan->copied[slot]));  // the setting before the last three has been copied
     plan->set = false;
+    if (!writable) plan->build.writes.clear();  // a captured write, replayed, leaves shared pages alone
     const size_t bytes = pack(plan->build, plan->staging[slot], &plan->head);
     DM_HIP(hipMemcpyAsync(plan->lists, plan->staging[slot], bytes, hipMemcpyHostToDevice, pool->ctx->stream));
     DM_HIP(hipEventRecord(plan->copied[slot], pool->ctx->stream));
@@ -662,7 +667,7 @@ int dmhip_attention_pages_device(dmhip_ctx *ctx, const dmhip_kv_plan *plan, size
     DM_REQUIRE_PTR(plan);
     DM_CHECK_STATUS(plan_checks(ctx, plan, layer));
     const dmhip_kv_pages *pool = plan->pool;
-    if (!isfinite(scale) || scale <= 0.0f) return fail_positive("attention scale");
+    if (!(scale > 0.0f && scale < 0x1p127f)) return fail_positive("attention scale");
     const size_t width = (size_t)plan->query_heads * pool->head_dim;
     if (query_stride < width) return fail_vector_length("paged attention", "query stride", width, query_stride);
     if (output_stride < width) return fail_vector_length("paged attention", "output stride", width, output_stride);
@@ -687,7 +692,7 @@ int dmhip_attention_pages_device(dmhip_ctx *ctx, const dmhip_kv_plan *plan, size
     call.out_type = plan->output_type;
     call.group = plan->shape.group;
     call.window = (uint32_t)plan->shape.window;
-    call.scale = scale * 1.44269504088896340736f;
+    call.scale = scale * 1.44269504088896340736f;  // finite below 2^127
     call.part_o = plan->part_o;
     call.part_ml = plan->part_ml;
     call.bad = attention_device_flag(ctx);

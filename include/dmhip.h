@@ -603,7 +603,8 @@ int dmhip_kv_pages_compact(dmhip_kv_pages *pool, size_t *moved);
    16-bit output and split for F32 output into three values (BF16) or two (F16),
    which leaves an error of 2^-24 or 2^-22 of it.  Sums, and the softmax's
    statistics, are 32-bit.  Holds device memory for max_tokens tokens a step
-   (and nothing grows later). */
+   (and nothing grows later).  VectorTooLarge: query_heads / kv_heads times
+   max_tokens from 2^30, or lists of the step's work from 2^32 bytes. */
 int dmhip_new_kv_plan(dmhip_kv_pages *pool, size_t query_heads, int has_window, size_t sliding_window,
                       uint32_t query_type, uint32_t output_type, size_t max_tokens, dmhip_kv_plan **out);
 /* Waits for the context's stream first.  Graphs that hold calls of the plan, or
@@ -632,14 +633,15 @@ int dmhip_kv_pages_write_device(dmhip_ctx *ctx, const dmhip_kv_plan *plan, size_
    reads KV head h / (query_heads / kv_heads).  Row t of the queries, [query_heads]
    [head_dimension], stands at t * query_stride values, that of the outputs at
    t * output_stride; they must not overlap.  Values in positions that a token
-   does not see never reach it, whatever they are.  scale: finite and positive
-   (InvalidPositiveParameter).  A row whose scores hold a NaN or +inf, or only
+   does not see never reach it, whatever they are.  scale: finite and positive,
+   below 2^127 (InvalidPositiveParameter).  A row whose scores hold a NaN or +inf, or only
    -inf, is reported by dmhip_attention_result (NonFinite "softmax") and not
    meaningful.  Refusals otherwise as dmhip_kv_pages_write_device.
 
    Stream-ordered; may be captured.  A captured call works, when it is
    replayed, on what the plan was last set to, and is not checked against the
-   sequences again: set the plan for each step, and replay on the context's
+   sequences again (a write does nothing where an eager one would refuse shared
+   pages): set the plan for each step, and replay on the context's
    stream or ordered with it.  The plan holds the work space of the call, so
    calls of one plan must not run at the same time.  dmhip_attention_result
    reports a replayed call only until the first result after its capture. */

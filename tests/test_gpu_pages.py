@@ -670,6 +670,30 @@ def test_captured_steps_follow_the_plan(ctx, kind, out_type):
     m.close()
 
 
+def test_a_replayed_write_leaves_shared_pages_alone(ctx):
+    rng = np.random.default_rng(19)
+    m = Model(ctx, BF16, 2, 16, pages=20, sequences=6)
+    root = m.new()
+    m.grow([root], [128], rng)
+    a, b = m.fork([root] * 2, [128, 128])
+    plan = m.pages.new_plan(2, None, F32, F32, 4)
+    k = m.device(rng.standard_normal((4, 32)).astype(np.float32))
+    m.pages.extend([a], [1])
+    plan.set([a], [1])
+    with Graph(ctx) as graph:
+        ctx.write_kv_pages_device(plan, 0, F32, k, 32, k, 32)
+    m.pages.truncate(a, 128)
+    for _ in range(3):
+        plan.set([a, b], [2, 2])  # the root's own pages
+        expect_error("InvalidArgument", ctx.write_kv_pages_device, plan, 0, F32, k, 32, k, 32)
+        graph.replay()
+        ctx.synchronize()
+        m.check_stored()
+    plan.free()
+    graph.free()
+    m.close()
+
+
 def test_a_plan_is_refused_once_its_sequences_have_changed(ctx):
     m = Model(ctx, BF16, 1, 8, sequences=6)
     a, b, other = m.new(), m.new(), m.new()
@@ -743,7 +767,8 @@ def test_refusals(ctx):
     for args, variant in [((3, None, F32, F32, 9), "InvalidAttentionShape"), ((0, None, F32, F32, 9), "InvalidAttentionShape"),
                           ((4, 0, F32, F32, 9), "EmptyInput"), ((4, None, F16, F32, 9), "UnsupportedTensorType"),
                           ((4, None, F32, 12, 9), "UnsupportedTensorType"), ((4, None, F32, F32, 0), "EmptyInput"),
-                          ((4, None, F32, F32, 2 ** 30), "VectorTooLarge")]:
+                          ((4, None, F32, F32, 2 ** 30), "VectorTooLarge"),
+                          ((2, None, F32, F32, 2 ** 30 - 1), "VectorTooLarge")]:  # lists of 6 GiB
         expect_error(variant, p.new_plan, *args)
     plan = p.new_plan(4, None, F32, BF16, 9)
     expect_error("EmptyInput", plan.set, [a], [0])
@@ -757,6 +782,7 @@ def test_refusals(ctx):
     ok = (plan, 1, 1.0, buf, 64, buf + 32768, 64)
     for i, value, variant in [(1, 2, "InvalidLayer"), (2, 0.0, "InvalidPositiveParameter"), (2, -1.0, "InvalidPositiveParameter"),
                               (2, float("nan"), "InvalidPositiveParameter"), (2, float("inf"), "InvalidPositiveParameter"),
+                              (2, 2.0 ** 127, "InvalidPositiveParameter"),
                               (3, 0, "InvalidArgument"), (3, buf + 2, "InvalidArgument"), (4, 63, "InvalidVectorLength"),
                               (5, 0, "InvalidArgument"), (5, buf + 1, "InvalidArgument"), (6, 63, "InvalidVectorLength")]:
         args = list(ok)

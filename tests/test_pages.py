@@ -434,3 +434,21 @@ def test_short_units_that_are_at_work_at_once_go_to_the_smallest_kernel(lib, tok
     finally:
         lib.shorts(0, 0)
     c.close()
+
+
+@pytest.mark.parametrize("deep,count", [(31, 32), (32, 32), (33, 32), (60, 32)])
+def test_prefixes_within_prefixes_are_shared_so_far(lib, deep, count):
+    c = Cache(lib, 1000, 80, 9000)
+    c.create()
+    c.extend([0], [2 * PAGE])
+    chain = [0]
+    for _ in range(deep):
+        c.fork([chain[-1]], [len(c.tokens[chain[-1]])])
+        chain.append(max(c.tokens))
+        c.extend([chain[-1]], [2 * PAGE])
+    c.extend(chain, [1] * len(chain))
+    check_plan(lib, c, chain, [1] * len(chain), 2, 2, 0, [16, 64, 128], [64] * 3, [64] * 3, 2, 10 ** 9, 10 ** 9)
+    units = np.concatenate([lists(lib, c.b, k, 8) for k in range(3)])
+    starts = {(u[0], u[3]) for u in units if u[1] > 2}  # of levels that several sequences share
+    assert len(starts) >= min(deep, count)
+    c.close()
