@@ -79,28 +79,35 @@ struct WriteCall {
     uint32_t source_type;
 };
 
-// Rows of keys (z = 0) or values (z = 1) into pages: a workgroup takes one
-// run of a page for one head, 32 slots at a time through LDS, so that rows are
-// read and pages written 16 bytes a lane.  Value chunks of which the run
+// Rows of keys (z even) or values (z odd) into pages: a workgroup takes one
+// run of a page for up to 128 dims of a head, 32 slots at a time through LDS, so
+// that rows are read and pages written 16 bytes a lane.  Value chunks of which the run
 // holds only some tokens are written a value at a time.  Bound by memory: 6874
-// F32 rows of 8 x 128 to BF16 pages 16 us, 5.2 TB/s, as a large copy.
+// F32 rows of 8 x 128 to BF16 pages 16 us, 5.2 TB/s, as a large copy; or, of few
+// runs, by one after another: 40 rows of 2 x 512 take 4 us less than with all of
+// a head's dims in a workgroup (46.5 against 50.6 with the attention), 4100 of
+// 8 x 256 0.7 us more of 136.
+constexpr uint32_t kWriteDims = 128;
 template <typename T>
 __global__ __launch_bounds__(256) void write_pages_kernel(WriteCall c) {
-    extern __shared__ __attribute__((aligned(16))) uint16_t tile[];  // [32][head_dim + 8]
+    constexpr uint32_t pitch = kWriteDims + 8;
+    __shared__ __attribute__((aligned(16))) uint16_t tile[32 * pitch];
     const PlanHeader &head = *(const PlanHeader *)c.plan;
     const WriteRun *runs = (const WriteRun *)(c.plan + head.write_at);
-    const uint32_t hd = c.kv.head_dim, h = blockIdx.y, values = blockIdx.z, pitch = hd + 8, eights = hd / 8;
+    const uint32_t hd = c.kv.head_dim, h = blockIdx.y, values = blockIdx.z & 1;
+    const uint32_t d0 = (blockIdx.z >> 1) * kWriteDims, dims = min(kWriteDims, hd - d0), eights = dims / 8;
     const void *rows = c.rows[values];
     const uint64_t stride = c.stride[values];
     for (uint32_t i = blockIdx.x; i < head.write_count; i += gridDim.x) {
         const WriteRun r = runs[i];
         const uint32_t page = c.kv.table[r.word];
-        T *block = (T *)c.kv.base + ((uint64_t)page * c.kv.kv_heads + h) * 2 * hd * kPageTokens + values * hd * kPageTokens;
+        T *block = (T *)c.kv.base + ((uint64_t)page * c.kv.kv_heads + h) * 2 * hd * kPageTokens +
+                   (values ? hd * kPageTokens + d0 * 8 : d0 * kPageTokens);
         for (uint32_t s0 = r.slot0 & ~31u; s0 < r.slot0 + r.count; s0 += 32) {
             const uint32_t a = r.slot0 > s0 ? r.slot0 - s0 : 0, b = min(32u, r.slot0 + r.count - s0);
             for (uint32_t w = threadIdx.x; w < (b - a) * eights; w += 256) {
                 const uint32_t slot = a + w / eights, ch = w % eights;
-                const uint64_t at = (uint64_t)(r.token0 + s0 + slot - r.slot0) * stride + (uint64_t)h * hd + ch * 8;
+                const uint64_t at = (uint64_t)(r.token0 + s0 + slot - r.slot0) * stride + (uint64_t)h * hd + d0 + ch * 8;
                 u32x4 out;
                 if (c.source_type == kF32) {
                     const f32x4a4 x = *(const f32x4a4 *)((const float *)rows + at);
@@ -122,8 +129,8 @@ __global__ __launch_bounds__(256) void write_pages_kernel(WriteCall c) {
                             *(const u32x4 *)(tile + slot * pitch + ch * 8);
                 }
             } else {
-                for (uint32_t w = threadIdx.x; w < 4 * hd; w += 256) {
-                    const uint32_t chunk = w / hd, d = w % hd;
+                for (uint32_t w = threadIdx.x; w < 4 * dims; w += 256) {
+                    const uint32_t chunk = w / dims, d = w % dims;
                     const uint32_t t0 = 16 * (chunk >> 1) + 4 * (chunk & 1);  // tokens t0 .. + 3, t0 + 8 .. + 11
                     uint16_t *dst = (uint16_t *)block + ((uint64_t)((s0 / 8 + chunk) * hd + d)) * 8;
                     if (a <= t0 && b >= t0 + 12) {
@@ -652,11 +659,11 @@ int dmhip_kv_pages_write_device(dmhip_ctx *ctx, const dmhip_kv_plan *plan, size_
     DM_HIP(hipStreamIsCapturing(ctx->stream, &st));
     const uint32_t grid = st == hipStreamCaptureStatusNone ? std::min(plan->head.write_count, 1u << 20) : captured_grid(ctx);
     const WriteCall call{pool->view((uint32_t)layer), plan->lists, {keys, values}, {key_stride, value_stride}, source_type};
-    const uint32_t lds = 32 * (pool->head_dim + 8) * 2;
+    const dim3 wide(grid, pool->kv_heads, 2 * ((pool->head_dim + kWriteDims - 1) / kWriteDims));
     if (pool->type == kBF16)
-        write_pages_kernel<__bf16><<<dim3(grid, pool->kv_heads, 2), 256, lds, ctx->stream>>>(call);
+        write_pages_kernel<__bf16><<<wide, 256, 0, ctx->stream>>>(call);
     else
-        write_pages_kernel<_Float16><<<dim3(grid, pool->kv_heads, 2), 256, lds, ctx->stream>>>(call);
+        write_pages_kernel<_Float16><<<wide, 256, 0, ctx->stream>>>(call);
     DM_HIP(hipGetLastError());
     return DMHIP_OK;
 }
