@@ -19,56 +19,60 @@ namespace dm {
 typedef uint32_t u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 
-// Kernel arguments hold 4 KiB.
-constexpr uint32_t kRunsPerLaunch = 320, kPairsPerLaunch = 480;
-struct TableRuns {
+// What a launch does to the pages and the table: kernel arguments hold 4 KiB.
+constexpr uint32_t kPairsPerLaunch = 192, kRunsPerLaunch = 192;
+struct PageChange {
+    uint8_t *base;  // of the first layer of the launch
+    uint64_t layer_bytes;
+    uint32_t *table;
+    uint32_t page_bytes, words, pairs, runs, table_slices;
+    bool rename;  // table words that name a moved page name its new place: pairs ascend in src
+    PagePair pair[kPairsPerLaunch];
     TableRun run[kRunsPerLaunch];
 };
-struct PagePairs {
-    PagePair pair[kPairsPerLaunch];
-};
 
-__global__ __launch_bounds__(64) void table_runs_kernel(uint32_t *table, TableRuns runs) {
-    const TableRun r = runs.run[blockIdx.x];
-    for (uint32_t i = threadIdx.x; i < r.count; i += 64)
-        table[r.at + i] = r.value & kTableCopy ? table[(r.value & ~kTableCopy) + i] : r.value + i;
-}
-
-// Table words that name a moved page name its new place: pairs ascend in src.
-__global__ __launch_bounds__(256) void table_moves_kernel(uint32_t *table, uint32_t words, PagePairs pairs,
-                                                          uint32_t count) {
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (uint64_t)gridDim.x * 256) {
-        const uint32_t page = table[i];
-        uint32_t lo = 0, hi = count;
+// Whole pages of every layer (z from table_slices on): 16 KiB a workgroup, four
+// 16-byte loads of a thread in flight; and beside them (z below) the table.
+// Bound by memory: 64 pages of 32 layers of 8 x 128, 2 x 537 MB, 129 us; of few
+// pages by the launch and the host: 4 branches of 8 layers, forked, released and
+// compacted, 25 us with launches of their own for the table, 18 so.
+constexpr uint32_t kCopyBytes = 16384;
+__global__ __launch_bounds__(256) void change_pages_kernel(PageChange c) {
+    if (blockIdx.z >= c.table_slices) {
+        const PagePair p = c.pair[blockIdx.y];
+        uint8_t *layer = c.base + (blockIdx.z - c.table_slices) * c.layer_bytes;
+        const uint8_t *src = layer + (uint64_t)p.src * c.page_bytes;
+        uint8_t *dst = layer + (uint64_t)p.dst * c.page_bytes;
+        const uint32_t at = blockIdx.x * kCopyBytes + threadIdx.x * 16;
+        u32x4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (at + i * 4096 < c.page_bytes) v[i] = *(const u32x4 *)(src + at + i * 4096);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (at + i * 4096 < c.page_bytes) *(u32x4 *)(dst + at + i * 4096) = v[i];
+        return;
+    }
+    const uint32_t block = (blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+    const uint32_t blocks = c.table_slices * gridDim.y * gridDim.x;
+    for (uint32_t k = block; k < c.runs; k += blocks) {
+        const TableRun r = c.run[k];
+        for (uint32_t i = threadIdx.x; i < r.count; i += 256)
+            c.table[r.at + i] = r.value & kTableCopy ? c.table[(r.value & ~kTableCopy) + i] : r.value + i;
+    }
+    if (!c.rename) return;
+    for (uint64_t i = (uint64_t)block * 256 + threadIdx.x; i < c.words; i += (uint64_t)blocks * 256) {
+        const uint32_t page = c.table[i];
+        uint32_t lo = 0, hi = c.pairs;
         while (lo < hi) {
             const uint32_t mid = (lo + hi) / 2;
-            if (pairs.pair[mid].src < page)
+            if (c.pair[mid].src < page)
                 lo = mid + 1;
             else
                 hi = mid;
         }
-        if (lo < count && pairs.pair[lo].src == page) table[i] = pairs.pair[lo].dst;
+        if (lo < c.pairs && c.pair[lo].src == page) c.table[i] = c.pair[lo].dst;
     }
-}
-
-// Whole pages of every layer: 16 KiB a workgroup, four 16-byte loads of a
-// thread in flight.  Bound by memory: 64 pages of 32 layers of 8 x 128, 2 x 537
-// MB, 129 us.
-constexpr uint32_t kCopyBytes = 16384;
-__global__ __launch_bounds__(256) void copy_pages_kernel(uint8_t *base, uint64_t layer_bytes, uint32_t page_bytes,
-                                                         PagePairs pairs) {
-    const PagePair p = pairs.pair[blockIdx.y];
-    uint8_t *layer = base + blockIdx.z * layer_bytes;
-    const uint8_t *src = layer + (uint64_t)p.src * page_bytes;
-    uint8_t *dst = layer + (uint64_t)p.dst * page_bytes;
-    const uint32_t at = blockIdx.x * kCopyBytes + threadIdx.x * 16;
-    u32x4 v[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (at + i * 4096 < page_bytes) v[i] = *(const u32x4 *)(src + at + i * 4096);
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (at + i * 4096 < page_bytes) *(u32x4 *)(dst + at + i * 4096) = v[i];
 }
 
 struct WriteCall {
@@ -155,7 +159,7 @@ __global__ __launch_bounds__(256) void write_pages_kernel(WriteCall c) {
     }
 }
 
-const void *module_anchor_kv_pages() { return (const void *)table_runs_kernel; }
+const void *module_anchor_kv_pages() { return (const void *)change_pages_kernel; }
 
 }  // namespace dm
 
@@ -234,43 +238,33 @@ static int refuse_capture(dmhip_ctx *ctx, const char *what) {
     return DMHIP_OK;
 }
 
-static int enqueue_copies(dmhip_kv_pages *p) {
+// The copies of pages and the changes of the table that the book asks for.
+static int enqueue_work(dmhip_kv_pages *p, bool rename) {
     const std::vector<PagePair> &copies = p->work.copies;
-    for (size_t i = 0; i < copies.size(); i += kPairsPerLaunch) {
-        const uint32_t n = (uint32_t)std::min<size_t>(kPairsPerLaunch, copies.size() - i);
-        PagePairs args;
-        memcpy(args.pair, copies.data() + i, n * sizeof(PagePair));
+    const std::vector<TableRun> &tables = p->work.tables;
+    PageChange c;
+    c.layer_bytes = p->layer_bytes;
+    c.table = p->table;
+    c.page_bytes = p->page_bytes;
+    c.words = p->book.sequences() * p->book.row();
+    c.rename = rename;
+    for (size_t i = 0, k = 0; i < copies.size() || k < tables.size(); i += c.pairs, k += c.runs) {
+        c.pairs = (uint32_t)std::min<size_t>(kPairsPerLaunch, copies.size() - i);
+        c.runs = (uint32_t)std::min<size_t>(kRunsPerLaunch, tables.size() - k);
+        memcpy(c.pair, copies.data() + i, c.pairs * sizeof(PagePair));
+        memcpy(c.run, tables.data() + k, c.runs * sizeof(TableRun));
+        const uint32_t x = c.pairs ? (p->page_bytes + kCopyBytes - 1) / kCopyBytes : 1, y = std::max(1u, c.pairs);
+        // four words of the table a thread, or a run a workgroup
+        const uint64_t wanted = std::max<uint64_t>(rename ? ((uint64_t)c.words + 1023) / 1024 : 0, c.runs);
+        const uint32_t slices = (uint32_t)std::min<uint64_t>(1024, (wanted + (uint64_t)x * y - 1) / ((uint64_t)x * y));
         for (uint32_t layer = 0; layer < p->layers; layer += 32768) {
-            const uint32_t layers = std::min(p->layers - layer, 32768u);
-            copy_pages_kernel<<<dim3((p->page_bytes + kCopyBytes - 1) / kCopyBytes, n, layers), 256, 0, p->ctx->stream>>>(
-                p->data + layer * p->layer_bytes, p->layer_bytes, p->page_bytes, args);
+            c.base = p->data + layer * p->layer_bytes;
+            c.table_slices = layer == 0 ? slices : 0;
+            const uint32_t layers = c.pairs ? std::min(p->layers - layer, 32768u) : 0;
+            if (layers + c.table_slices == 0) break;
+            change_pages_kernel<<<dim3(x, y, layers + c.table_slices), 256, 0, p->ctx->stream>>>(c);
             DM_HIP(hipGetLastError());
         }
-    }
-    return DMHIP_OK;
-}
-
-static int enqueue_tables(dmhip_kv_pages *p) {
-    const std::vector<TableRun> &runs = p->work.tables;
-    for (size_t i = 0; i < runs.size(); i += kRunsPerLaunch) {
-        const uint32_t n = (uint32_t)std::min<size_t>(kRunsPerLaunch, runs.size() - i);
-        TableRuns args;
-        memcpy(args.run, runs.data() + i, n * sizeof(TableRun));
-        table_runs_kernel<<<n, 64, 0, p->ctx->stream>>>(p->table, args);
-        DM_HIP(hipGetLastError());
-    }
-    return DMHIP_OK;
-}
-
-static int enqueue_moves(dmhip_kv_pages *p) {
-    const std::vector<PagePair> &moves = p->work.copies;
-    const uint32_t words = p->book.sequences() * p->book.row();
-    for (size_t i = 0; i < moves.size(); i += kPairsPerLaunch) {
-        const uint32_t n = (uint32_t)std::min<size_t>(kPairsPerLaunch, moves.size() - i);
-        PagePairs args;
-        memcpy(args.pair, moves.data() + i, n * sizeof(PagePair));
-        table_moves_kernel<<<std::min((words + 255) / 256, 2048u), 256, 0, p->ctx->stream>>>(p->table, words, args, n);
-        DM_HIP(hipGetLastError());
     }
     return DMHIP_OK;
 }
@@ -486,8 +480,7 @@ int dmhip_kv_sequences_extend(dmhip_kv_pages *pool, size_t count, const size_t *
     DM_CHECK_STATUS(set_device(pool->ctx));
     DM_CHECK_STATUS(refuse_capture(pool->ctx, "extending KV sequences"));
     DM_HOST_MEMORY(DM_CHECK_STATUS(refuse(pool, pool->book.extend(count, sequences, tokens, &pool->work))));
-    DM_CHECK_STATUS(enqueue_copies(pool));
-    return enqueue_tables(pool);
+    return enqueue_work(pool, false);
 }
 
 int dmhip_kv_sequences_fork(dmhip_kv_pages *pool, size_t count, const size_t *parents, const size_t *lengths,
@@ -500,8 +493,7 @@ int dmhip_kv_sequences_fork(dmhip_kv_pages *pool, size_t count, const size_t *pa
     DM_CHECK_STATUS(set_device(pool->ctx));
     DM_CHECK_STATUS(refuse_capture(pool->ctx, "forking KV sequences"));
     DM_HOST_MEMORY(DM_CHECK_STATUS(refuse(pool, pool->book.fork(count, parents, lengths, children, &pool->work))));
-    DM_CHECK_STATUS(enqueue_copies(pool));
-    return enqueue_tables(pool);
+    return enqueue_work(pool, false);
 }
 
 int dmhip_kv_pages_compact(dmhip_kv_pages *pool, size_t *moved) {
@@ -510,8 +502,7 @@ int dmhip_kv_pages_compact(dmhip_kv_pages *pool, size_t *moved) {
     DM_CHECK_STATUS(refuse_capture(pool->ctx, "compacting KV pages"));
     DM_HOST_MEMORY(pool->book.compact(&pool->work));
     if (moved) *moved = pool->work.copies.size();
-    DM_CHECK_STATUS(enqueue_copies(pool));
-    return enqueue_moves(pool);
+    return enqueue_work(pool, true);
 }
 
 int dmhip_new_kv_plan(dmhip_kv_pages *pool, size_t query_heads, int has_window, size_t sliding_window,
